@@ -1,0 +1,246 @@
+"""The decoder operators without a GPU: what the header declares is exported and bound, every refusal, what becomes which
+kernel, and the lengths a cache keeps on the host.  On a plan-only device kernels are compiled and nothing is computed."""
+import ctypes
+import os
+import re
+
+import numpy as np
+import pytest
+
+from helpers import ROOT
+
+F16, F32 = np.float16, np.float32
+
+
+def zeros(w, dev, shape, dtype=F32):
+    return w.Tensor.new(dev, np.zeros(shape, dtype))
+
+
+def weights(w, dev, k=64, n=16, group=32, **more):
+    g = -(-k // group)
+    return w.Q4Weights(dev, np.zeros((k, n), np.uint8), np.ones((g, n), F16), group=group, **more)
+
+
+def refused(w, match):
+    return pytest.raises(w.WkfError, match=match)
+
+
+def test_header_library_and_binding_agree(wkf):
+    text = open(os.path.join(ROOT, "include", "wkf_decode.h")).read()
+    declared = set(re.findall(r"\b(wkf_[a-z0-9_]+)\s*\(", re.sub(r"/\*.*?\*/", "", text, flags=re.S)))
+    assert declared == set(wkf.DECODE_EXPORTS)
+    lib = ctypes.CDLL(wkf.LIB_PATH)
+    assert not [n for n in sorted(declared) if not hasattr(lib, n)]
+
+
+def test_null_arguments_are_refused(wkf, planner):
+    lib, h = wkf.load(), ctypes.c_void_p()
+    out = ctypes.byref(h)
+    t = zeros(wkf, planner, (2, 4, 64))
+    cache, q4 = wkf.KvCache(planner, 1, 2, 64, 64), weights(wkf, planner)
+    one = (ctypes.c_size_t * 4)(1, 1, 1, 1)
+    for rc in (lib.wkf_tensor_zeros(None, 0, 1, one, out), lib.wkf_tensor_zeros(planner._h, 0, 1, one, None), lib.wkf_tensor_zeros(planner._h, 0, 1, None, out),
+               lib.wkf_tensor_materialize_into(None, 1, None), lib.wkf_tensor_device_ptr(None, out), lib.wkf_tensor_device_ptr(t._h, None),
+               lib.wkf_q4_new(planner._h, 32, 16, 32, None, 0, None, None, out), lib.wkf_q4_shape(None, one, one, one),
+               lib.wkf_tensor_mat_mul_q4(None, q4._h, out), lib.wkf_tensor_mat_mul_q4(t._h, None, out), lib.wkf_tensor_mat_mul_q4(t._h, q4._h, None),
+               lib.wkf_tensor_norm_rope(t._h, None, None, None, 0.0, None, out), lib.wkf_kv_cache_create(None, 1, 1, 64, 64, 32, out),
+               lib.wkf_kv_cache_create(planner._h, 1, 1, 64, 64, 32, None), lib.wkf_kv_cache_length(None, 0, one), lib.wkf_kv_cache_length(cache._h, 0, None),
+               lib.wkf_kv_cache_reset(None, 0), lib.wkf_kv_cache_append(cache._h, None, t._h, None), lib.wkf_kv_cache_append(None, t._h, t._h, None),
+               lib.wkf_kv_cache_values(None, 0, 0, 1, out), lib.wkf_kv_cache_values(cache._h, 0, 0, 1, None), lib.wkf_tensor_attend(None, cache._h, 1.0, 1, None, out),
+               lib.wkf_tensor_attend(t._h, None, 1.0, 1, None, out), lib.wkf_tensor_attend(t._h, cache._h, 1.0, 1, None, None)):
+        assert rc == wkf.ERR_INVALID_ARG
+    lib.wkf_q4_free(None)
+    lib.wkf_kv_cache_free(None)
+
+
+def test_refusals_of_zeros_and_materialize_into(wkf, planner):
+    a, b = zeros(wkf, planner, (3, 4)), zeros(wkf, planner, (3, 4))
+    with refused(wkf, "dtype"):
+        wkf.Tensor.zeros(planner, (3,), 7)
+    with refused(wkf, "too large"):
+        wkf.Tensor.zeros(planner, (1 << 40, 1 << 40))
+    with refused(wkf, "no tensors"):
+        wkf.materialize_into([], [])
+    with refused(wkf, "one output per tensor"):
+        wkf.materialize_into([a], [])
+    with refused(wkf, "lazy expression"):
+        wkf.materialize_into([a], [b + 1.0])
+    with refused(wkf, "lazy expression"):
+        wkf.materialize_into([a.narrow(0, 0, 2)], [b.narrow(0, 0, 2)])
+    with refused(wkf, "shape and dtype"):
+        wkf.materialize_into([a], [zeros(wkf, planner, (4, 3))])
+    with refused(wkf, "shape and dtype"):
+        wkf.materialize_into([a], [zeros(wkf, planner, (3, 4), F16)])
+    with refused(wkf, "the same tensor"):
+        wkf.materialize_into([a + 1.0, a + 2.0], [b, b.clone()])
+    other = wkf.Device.planner()
+    with refused(wkf, "different devices"):
+        wkf.materialize_into([a], [zeros(wkf, other, (3, 4))])
+    with refused(wkf, "hold data"):
+        (a + 1.0).device_ptr()
+    assert a.device_ptr() and not hasattr(a, "__cuda_array_interface__")
+    assert wkf.Tensor.zeros(planner, (0, 5)).shape() == (0, 5) and wkf.Tensor.zeros(planner, ()).rank() == 0
+
+
+def test_refusals_of_weights_in_4_bits(wkf, planner):
+    codes, scales = np.zeros((64, 16), np.uint8), np.ones((2, 16), F16)
+    for bad, match in [(dict(codes=codes + 16), "0 .. 15"), (dict(codes=codes.astype(int) - 1), "0 .. 15"), (dict(codes=codes.astype(F32)), "whole numbers"),
+                       (dict(codes=codes[:0]), "whole numbers"), (dict(codes=codes[0]), "matrix"), (dict(scales=scales[:1]), "scales"),
+                       (dict(scales=scales.astype(np.float64)), "scales"), (dict(zeros=np.full((2, 16), 16)), "zeros"), (dict(zeros=np.zeros((1, 16), int)), "zeros"),
+                       (dict(group=48), "multiple of 32"), (dict(group=0), "multiple of 32"), (dict(group=-32), "multiple of 32")]:
+        with refused(wkf, match):
+            wkf.Q4Weights(planner, **{"codes": codes, "scales": scales, "group": 32, **bad})
+    lib, h = wkf.load(), ctypes.c_void_p()
+    wrong = codes + 16
+    p = lambda a: a.ctypes.data_as(ctypes.c_void_p)  # noqa: E731
+    for args in ((0, 16, 32, p(codes), 1, p(scales), None), (64, 0, 32, p(codes), 1, p(scales), None), (64, 16, 33, p(codes), 1, p(scales), None),
+                 (64, 16, 32, p(wrong), 1, p(scales), None), (64, 16, 32, p(codes), 1, p(scales), p(wrong)), (64, 16, 32, p(codes), 2, p(scales), None),
+                 (1 << 40, 1 << 40, 32, p(codes), 1, p(scales), None)):
+        assert lib.wkf_q4_new(planner._h, *args, ctypes.byref(h)) == wkf.ERR_INVALID_ARG
+    w = weights(wkf, planner)
+    with refused(wkf, "last dimension"):
+        zeros(wkf, planner, (3, 63)).mat_mul_q4(w)
+    with refused(wkf, "last dimension"):
+        zeros(wkf, planner, ()).mat_mul_q4(w)
+    with refused(wkf, "different devices"):
+        zeros(wkf, wkf.Device.planner(), (3, 64)).mat_mul_q4(w)
+    y = zeros(wkf, planner, (2, 3, 64), F16).mat_mul_q4(w)
+    assert y.shape() == (2, 3, 16) and y.datatype() == wkf.F16
+    assert zeros(wkf, planner, (64,)).mat_mul_q4(w).shape() == (16,)
+
+
+def test_refusals_of_norm_rope(wkf, planner):
+    t, g, c = zeros(wkf, planner, (2, 3, 5, 8), F16), zeros(wkf, planner, (8,), F16), zeros(wkf, planner, (9, 4))
+    ok = dict(weight=g, cos=c, sin=c, eps=1e-5)
+    for bad, match in [(dict(weight=zeros(wkf, planner, (4,), F16)), "weight"), (dict(cos=zeros(wkf, planner, (9, 3))), "tables"), (dict(sin=zeros(wkf, planner, (8, 4))), "tables"),
+                       (dict(cos=zeros(wkf, planner, (9, 4), F16)), "differ in dtype"), (dict(eps=-1.0), "eps"), (dict(eps=float("nan")), "eps"), (dict(eps=float("inf")), "eps"),
+                       (dict(positions=[0]), "one position"), (dict(positions=[0, 5]), "tables end"), (dict(positions=[10, 0]), "tables end"),
+                       (dict(weight=zeros(wkf, wkf.Device.planner(), (8,), F16)), "different devices")]:
+        with refused(wkf, match):
+            t.norm_rope(**{**ok, **bad})
+    with refused(wkf, "expects"):
+        zeros(wkf, planner, (5, 8), F16).norm_rope(**ok)
+    with refused(wkf, "even"):
+        zeros(wkf, planner, (2, 5, 7)).norm_rope(**ok)
+    with refused(wkf, "even"):
+        zeros(wkf, planner, (1, 1, 1026)).norm_rope(**ok)
+    with refused(wkf, "dtype or f32"):
+        zeros(wkf, planner, (2, 5, 8)).norm_rope(**ok)
+    assert t.norm_rope(**ok, positions=[4, 0]).shape() == (2, 3, 5, 8)
+
+
+def test_refusals_of_the_cache_and_its_attention(wkf, planner):
+    for bad, match in [(dict(sequences=257), "sequences"), (dict(kv_heads=65536), "heads"), (dict(head_dim=257), "elements"), (dict(block=48), "block"), (dict(block=256), "block"),
+                       (dict(capacity=(1 << 30) + 1), "capacity"), (dict(sequences=0), "positive"), (dict(head_dim=-1), "positive"),
+                       (dict(sequences=256, kv_heads=65535, head_dim=256, capacity=1 << 30), "too large")]:
+        with refused(wkf, match):
+            wkf.KvCache(planner, **{"sequences": 2, "kv_heads": 2, "head_dim": 64, "capacity": 40, "block": 32, **bad})
+    lib, h = wkf.load(), ctypes.c_void_p()
+    assert lib.wkf_kv_cache_create(planner._h, 0, 2, 64, 40, 32, ctypes.byref(h)) == wkf.ERR_INVALID_ARG
+    cache = wkf.KvCache(planner, 2, 2, 64, 40, 32)
+    k = zeros(wkf, planner, (2, 2, 30, 64))
+    for args, match in [((zeros(wkf, planner, (2, 30, 64)), k), "sequences"), ((zeros(wkf, planner, (3, 2, 30, 64)), k), "sequences"), ((k, zeros(wkf, planner, (2, 4, 30, 64))), "heads"),
+                        ((k, zeros(wkf, planner, (2, 2, 29, 64))), "different numbers"), ((k, zeros(wkf, planner, (2, 2, 30, 32))), "elements"),
+                        ((k, zeros(wkf, planner, (2, 2, 30, 64), F16)), "dtype"), ((k, k, [30, 31]), "count"), ((k, k, [30]), "count per sequence"), ((k, k, [-1, 3]), "count per sequence"),
+                        ((k, zeros(wkf, wkf.Device.planner(), (2, 2, 30, 64))), "another device")]:
+        with refused(wkf, match):
+            cache.append(*args)
+    assert cache.lengths() == [0, 0]
+    cache.append(k, k, [30, 7])
+    with refused(wkf, "room for 40"):
+        cache.append(k, k, [0, 30]) or cache.append(k, k, [11, 0])
+    assert cache.lengths() == [30, 37]  # a refused append adds nothing, to no sequence
+    with refused(wkf, "room for 40"):
+        cache.append(k, k, [1, 4])
+    assert cache.lengths() == [30, 37]
+    q = zeros(wkf, planner, (2, 4, 31, 64), F16)
+    for t, more, match in [(q, {}, "fewer than"), (q, dict(counts=[32, 1]), "count"), (zeros(wkf, planner, (2, 3, 1, 64)), {}, "multiple"), (zeros(wkf, planner, (2, 0, 1, 64)), {}, "multiple"),
+                           (zeros(wkf, planner, (2, 4, 1, 65)), {}, "elements"), (zeros(wkf, planner, (4, 1, 64)), {}, "sequences"), (q, dict(counts=[1, 1], scale=-1.0), "scale"),
+                           (q, dict(counts=[1, 1], scale=float("nan")), "scale"), (q, dict(counts=[1, 1], scale=float("inf")), "scale"),
+                           (zeros(wkf, wkf.Device.planner(), (2, 4, 1, 64)), {}, "another device")]:
+        with refused(wkf, match):
+            t.attend(cache, **more)
+    for args in ((0, 41), (40, 1), (41, 0)):
+        with refused(wkf, "capacity"):
+            cache.values(*args)
+    with refused(wkf, "dtype"):
+        cache.values(0, 1, 5)
+    with refused(wkf, "no such sequence"):
+        cache.reset(2)
+    assert lib.wkf_kv_cache_reset(cache._h, 2) == wkf.ERR_INVALID_ARG and lib.wkf_kv_cache_length(cache._h, 2, ctypes.byref(ctypes.c_size_t())) == wkf.ERR_INVALID_ARG
+    one = wkf.KvCache(planner, 1, 2, 64, 40, 32)
+    one.append(zeros(wkf, planner, (2, 3, 64)), zeros(wkf, planner, (2, 3, 64)))
+    assert zeros(wkf, planner, (4, 2, 64)).attend(one).shape() == (4, 2, 64) and one.lengths() == [3]
+
+
+def test_a_node_stands_for_the_cache_it_was_recorded_with(wkf, planner):
+    cache = wkf.KvCache(planner, 1, 1, 64, 40, 32)
+    k = zeros(wkf, planner, (1, 1, 4, 64))
+    cache.append(k, k)
+    early = [zeros(wkf, planner, (1, 1, 1, 64)).attend(cache), cache.values()]
+    for t in early:
+        t.materialize()
+    cache.append(k, k, [0])  # nothing is appended: still the same cache
+    for t in early:
+        t.materialize()
+    cache.append(k, k)
+    for t in early:
+        with refused(wkf, "appended to or reset"):
+            t.materialize()
+    out = wkf.Tensor.zeros(planner, (1, 1, 1, 64))
+    with refused(wkf, "appended to or reset"):
+        wkf.materialize_into([early[0] * 2.0], [out])
+
+
+def test_handles_may_go_before_what_was_recorded_with_them(wkf, planner):
+    w, cache = weights(wkf, planner), wkf.KvCache(planner, 1, 1, 64, 40, 32)
+    k = zeros(wkf, planner, (1, 1, 4, 64))
+    cache.append(k, k)
+    y, o = zeros(wkf, planner, (3, 64)).mat_mul_q4(w), zeros(wkf, planner, (1, 2, 1, 64)).attend(cache)
+    del w, cache
+    y.materialize()
+    o.materialize()
+
+
+def test_a_device_may_go_before_its_cache_and_weights(wkf):
+    dev = wkf.Device.planner()
+    w, cache = weights(wkf, dev), wkf.KvCache(dev, 1, 1, 64, 40, 32)
+    dev.close()
+    del w, cache
+
+
+def test_what_becomes_which_kernel(wkf, planner):
+    x = zeros(wkf, planner, (3, 64), F16)
+    y = ((x * 2.0).mat_mul_q4(weights(wkf, planner)) + 1.0).exp()
+    y.materialize()
+    kinds = [k.kind for k in y.kernels()]
+    assert kinds[0] == "map" and kinds[-1] == "map" and "q4_mat_mul" in kinds[1:-1]
+    qk = zeros(wkf, planner, (2, 5, 6, 64))
+    g, c, d = zeros(wkf, planner, (64,)), zeros(wkf, planner, (9, 32)), zeros(wkf, planner, (9, 32))
+    q, k = qk.narrow(2, 0, 4).transpose(1, 2), qk.narrow(2, 4, 2).transpose(1, 2)
+    outs = [wkf.Tensor.zeros(planner, (2, 4, 5, 64)), wkf.Tensor.zeros(planner, (2, 2, 5, 64))]
+
+    def kinds_of(a, b):
+        wkf.materialize_into([a, b], outs)
+        return [n.kind for n in a.kernels()]
+
+    assert kinds_of(q.norm_rope(g, c, c, 1e-5, [1, 2]), k.norm_rope(g, c, c, 1e-5, [1, 2])) == ["norm_rope"]
+    # other positions, tables or eps: a launch each
+    assert kinds_of(q.norm_rope(g, c, c, 1e-5, [1, 2]), k.norm_rope(g, c, c, 1e-5, [1, 3])) == ["norm_rope"] * 2
+    assert kinds_of(q.norm_rope(g, c, c, 1e-5), k.norm_rope(g, d, c, 1e-5)) == ["norm_rope"] * 2
+    assert kinds_of(q.norm_rope(g, c, c, 1e-5), k.norm_rope(g, c, c, 1e-6)) == ["norm_rope"] * 2
+    # a value that is not an operator's own is computed and copied
+    assert kinds_of(q.norm_rope(g, c, c, 1e-5) * 2.0, k.norm_rope(g, c, c, 1e-5)).count("norm_rope") == 2
+    dot = q.norm_rope(g, c, c, 1e-5).graphvis()
+    assert "norm_rope ([2, 4, 5, 64] f32)" in dot and dot.count("->") >= 4
+
+
+def test_extern_block_of_the_guide_matches_the_header():
+    """The integration guide declares every function of wkf_decode.h with as many arguments."""
+    text = re.sub(r"/\*.*?\*/", " ", open(os.path.join(ROOT, "include", "wkf_decode.h")).read(), flags=re.S)
+    c = {m.group(1): m.group(2).count(",") + 1 for m in re.finditer(r"(?:int|void)\s+(wkf_\w+)\s*\(([^;{]*?)\)\s*;", text)}
+    guide = open(os.path.join(ROOT, "INTEGRATION.md")).read()
+    block = guide[guide.index("// src/ffi_decode.rs"):]
+    block = block[:block.index("```")]
+    rust = {m.group(1): len([p for p in m.group(2).split(",") if p.strip()]) for m in re.finditer(r"pub fn (wkf_\w+)\s*\(([^)]*)\)", block)}
+    assert rust == c

@@ -12,11 +12,11 @@ flags=(-O2 -std=c++17 -fPIC -Wall -Wno-unused-function -Wno-unused-value -Wno-un
 hipcc "${flags[@]}" --offload-arch=gfx950 -Xclang -target-feature -Xclang -packed-fp32-ops -x hip -c hip_ffi.cpp -o "$obj/hip_ffi.o" \
   2> >(grep -v "packed-fp32-ops' is not a recognized feature" >&2)
 pids=()
-for f in core codegen graph gemm tensor_api; do
+for f in core codegen graph gemm decode tensor_api decode_api; do
   hipcc "${flags[@]}" -x c++ -c "$f.cpp" -o "$obj/$f.o" &
   pids+=($!)
 done
 for p in "${pids[@]}"; do wait "$p"; done
-hipcc --hip-link --offload-arch=gfx950 -shared -fPIC "$obj"/hip_ffi.o "$obj"/core.o "$obj"/codegen.o "$obj"/graph.o "$obj"/gemm.o "$obj"/tensor_api.o \
+hipcc --hip-link --offload-arch=gfx950 -shared -fPIC "$obj"/hip_ffi.o "$obj"/core.o "$obj"/codegen.o "$obj"/graph.o "$obj"/gemm.o "$obj"/decode.o "$obj"/tensor_api.o "$obj"/decode_api.o \
   -o "$here/libwkf_hip.so" -lhiprtc -Wl,-rpath,/opt/rocm/lib
 echo "built $here/libwkf_hip.so"

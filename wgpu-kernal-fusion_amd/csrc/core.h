@@ -95,12 +95,18 @@ struct TensorData {
 // mergeable graph object (src/compute_graph/mod.rs:20-276).  Here a node owns
 // its parents through shared pointers, so there is nothing to merge when two
 // tensors meet and a node dies with its last handle.
-enum class NodeKind { Tensor, ElementWise, PairWise, Reduce, MatMul, MapLayout, Resize, SliceAssign };
+enum class NodeKind { Tensor, ElementWise, PairWise, Reduce, MatMul, MapLayout, Resize, SliceAssign,
+                      MatMulQ4, NormRope, CacheValues, Attend };  // the last four: decode.h
 
 struct Node;
 using NodeP = std::shared_ptr<Node>;
 
 enum class MapKind { Slice, Transpose, Broadcast };
+
+// What a decoder operator's node carries besides its inputs (decode.h).
+struct DecodeArgs {
+  virtual ~DecodeArgs() = default;
+};
 
 struct Node {
   NodeKind kind;
@@ -116,6 +122,8 @@ struct Node {
   size_t axis0 = 0, axis1 = 0;                    // MapLayout::Transpose; Broadcast: axis0 = inserted dim
   std::vector<size_t> new_shape, fill_shape;      // Resize (src/resize.rs:12-26); Broadcast: new_shape
   TensorData data;                                // Tensor leaf
+  std::vector<NodeP> more;                        // further inputs (NormRope: weight, cos, sin)
+  std::shared_ptr<const DecodeArgs> decode;       // MatMulQ4, NormRope, CacheValues, Attend
 };
 
 // ---- fused expression program ---------------------------------------------

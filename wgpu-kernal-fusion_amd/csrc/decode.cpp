@@ -1,0 +1,378 @@
+// The decoder operators' launches: which kernel a node becomes and what it is given.  The kernels are in kernels/.
+#include "decode.h"
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <sstream>
+
+#include "graph.h"
+
+namespace wkf {
+
+namespace {
+const char* const kPrelude =
+#include "kernels/prelude.hip.inc"
+    ;
+const char* const kKvLayout =
+#include "kernels/kv_layout.hip.inc"
+    ;
+const char* const kKvAppend =
+#include "kernels/kv_append.hip.inc"
+    ;
+const char* const kKvValues =
+#include "kernels/kv_values.hip.inc"
+    ;
+const char* const kAttend =
+#include "kernels/attend.hip.inc"
+    ;
+const char* const kNormRope =
+#include "kernels/norm_rope.hip.inc"
+    ;
+const char* const kQ4Pack =
+#include "kernels/q4_pack.hip.inc"
+    ;
+const char* const kQ4MatMul =
+#include "kernels/q4_mat_mul.hip.inc"
+    ;
+
+char* ptr(const BufRef& b) { return static_cast<char*>(wkf_buffer_ptr(b.get())); }
+// the first element of a tensor's layout
+char* first(const TensorData& t) { return ptr(t.buffer) + t.layout.offset * dtype_size(t.dtype); }
+
+std::string define(const char* name, size_t v) { return std::string("#define ") + name + " " + std::to_string(v) + "\n"; }
+
+// Lengths of up to 8, 64 or 256 sequences travel in an argument block: three kernels, so that the usual few do not carry 2 KB.
+size_t room_for(size_t sequences) { return sequences <= 8 ? 8 : sequences <= 64 ? 64 : kMaxSequences; }
+
+uint32_t grid_dim(size_t v, const char* what) {
+  if (v > 0x7fffffffull) throw Error(WKF_ERR_UNSUPPORTED, std::string(what) + ": too many workgroups");
+  return uint32_t(v);
+}
+
+std::string kv_defines(const KvCache& c, DType dt, size_t nb) {
+  return define("WKF_H", dt == DType::F16) + define("D", c.dim) + define("DP", c.dp) + define("T", c.block) + define("NB", nb);
+}
+std::string kv_signature(const char* what, const KvCache& c, DType dt, size_t nb) {
+  std::ostringstream s;
+  s << what << "|gfx950|" << dtype_name(dt) << "|d" << c.dim << "|t" << c.block << "|nb" << nb;
+  return s.str();
+}
+}  // namespace
+
+// The value of `n` with its elements dense in row-major order, or at least its last dimension (`rows` true).
+TensorData Resolver::rows_dense(const NodeP& n) {
+  TensorData t = resolve(n);
+  const size_t R = t.layout.rank();
+  if (R && t.layout.shape[R - 1] > 1 && t.layout.strides[R - 1] != 1) return make_contiguous(t);
+  return t;
+}
+
+// ---- products with 4-bit weights ----------------------------------------------------------------
+
+void Resolver::pack_q4(Q4& w, const TensorData& codes, const TensorData& scales, const TensorData& zeros) {
+  const bool z = bool(zeros.buffer), sh = w.scale_dtype == DType::F16;
+  const std::string sig = std::string("q4_pack|gfx950|") + dtype_name(w.scale_dtype) + (z ? "|zeros" : "");
+  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + define("WKF_SH", sh) + define("WKF_Z", z) + kQ4Pack; });
+  struct {
+    const void *codes, *scales, *zeros;
+    void *out, *out_scales, *out_zeros;
+    uint32_t k, n, groups, tiles_k;
+  } a = {ptr(codes.buffer), ptr(scales.buffer), z ? ptr(zeros.buffer) : nullptr, ptr(w.codes), ptr(w.scales), z ? ptr(w.zeros) : nullptr,
+         uint32_t(w.k), uint32_t(w.n), uint32_t(w.groups), uint32_t(w.tiles_k())};
+  launch("q4_pack", sig, "", k, grid_dim(w.tiles_k() * w.tiles_n(), "q4"), 1, 1, 64, a);
+}
+
+TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
+  const Q4& w = *static_cast<const Q4Args&>(*n->decode).w;
+  TensorData x = resolve(n->a);
+  if (x.layout.strides != Layout::contiguous_strides(x.layout.shape)) x = make_contiguous(x);
+  TensorData out = result_of(n.get());
+  const size_t M = x.layout.numel() / w.k, N = w.n;
+  if (!M) return out;
+  if (M > 0xfffffull) throw Error(WKF_ERR_UNSUPPORTED, "mat_mul_q4: more than 2^20 rows");
+  const bool z = bool(w.zeros), h = x.dtype == DType::F16, sh = w.scale_dtype == DType::F16;
+  const std::string sig = std::string("q4_mat_mul|gfx950|") + dtype_name(x.dtype) + "|s" + dtype_name(w.scale_dtype) + (z ? "|zeros" : "");
+  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + define("WKF_H", h) + define("WKF_SH", sh) + define("WKF_Z", z) + kQ4MatMul; });
+  struct {
+    const void *x, *codes, *scales, *zeros;
+    void* y;
+    uint32_t m, n, k, group, groups, tiles_k;
+  } a = {first(x), ptr(w.codes), ptr(w.scales), z ? ptr(w.zeros) : nullptr, first(out),
+         uint32_t(M), uint32_t(N), uint32_t(w.k), uint32_t(w.group), uint32_t(w.groups), uint32_t(w.tiles_k())};
+  std::ostringstream d;
+  d << "m=" << M << " n=" << N << " k=" << w.k << " group=" << w.group;
+  launch("q4_mat_mul", sig, d.str(), k, uint32_t(w.tiles_n()), uint32_t((M + 15) / 16), 1, 256, a);
+  return out;
+}
+
+// ---- norm and rotation of heads -------------------------------------------------------------------
+
+namespace {
+constexpr size_t kMaxMembers = 4;  // tensors of one norm_rope launch
+
+const NormRopeArgs& norm_rope_args(const Node* n) { return static_cast<const NormRopeArgs&>(*n->decode); }
+
+// [batch, heads, seq, dim] of a rank-3 or rank-4 node
+size_t nr_dim(const Node* n, size_t i) {
+  const std::vector<size_t>& s = n->shape;
+  return s.size() == 4 ? s[i] : i == 0 ? 1 : s[i - 1];
+}
+}  // namespace
+
+void Resolver::join_norm_ropes(const std::vector<NodeP>& roots) {
+  std::vector<std::vector<const Node*>> groups;
+  std::set<const Node*> seen;
+  for (const NodeP& r : roots) {
+    if (r->kind != NodeKind::NormRope || !seen.insert(r.get()).second || materialized_.count(r.get())) continue;
+    bool placed = false;
+    for (auto& g : groups) {
+      const Node *o = g[0], *n = r.get();
+      const NormRopeArgs &x = norm_rope_args(o), &y = norm_rope_args(n);
+      if (g.size() < kMaxMembers && o->dtype == n->dtype && nr_dim(o, 0) == nr_dim(n, 0) && nr_dim(o, 2) == nr_dim(n, 2) && nr_dim(o, 3) == nr_dim(n, 3) &&
+          o->more[0]->dtype == n->more[0]->dtype && o->more[1] == n->more[1] && o->more[2] == n->more[2] &&
+          memcmp(&x.eps, &y.eps, sizeof(float)) == 0 && x.positions == y.positions) {
+        g.push_back(n);
+        placed = true;
+        break;
+      }
+    }
+    if (!placed) groups.push_back({r.get()});
+  }
+  for (auto& g : groups) {
+    if (g.size() < 2) continue;
+    std::vector<TensorData> outs = launch_norm_rope(g);
+    for (size_t i = 0; i < g.size(); i++) materialized_[g[i]] = outs[i];
+  }
+}
+
+TensorData Resolver::run_norm_rope(const NodeP& n) { return launch_norm_rope({n.get()})[0]; }
+
+std::vector<TensorData> Resolver::launch_norm_rope(const std::vector<const Node*>& members) {
+  const Node* n0 = members[0];
+  const NormRopeArgs& args = norm_rope_args(n0);
+  const size_t batch = nr_dim(n0, 0), seq = nr_dim(n0, 2), dim = nr_dim(n0, 3);
+  auto dense = [&](const NodeP& n) {
+    TensorData t = resolve(n);
+    return t.layout.strides == Layout::contiguous_strides(t.layout.shape) ? t : make_contiguous(t);
+  };
+  TensorData cos = dense(n0->more[1]), sin = dense(n0->more[2]);
+  std::vector<TensorData> xs, ws, outs;
+  size_t heads = 0;
+  for (const Node* n : members) {
+    xs.push_back(rows_dense(n->a));
+    ws.push_back(dense(n->more[0]));
+    outs.push_back(result_of(n));
+    heads += nr_dim(n, 1);
+  }
+  if (!batch || !seq || !heads) return outs;
+  const size_t nb = room_for(std::min(batch, kMaxSequences)), count = members.size();
+  const bool full = cos.layout.shape[1] == dim;
+  std::ostringstream sg;
+  sg << "norm_rope|gfx950|" << dtype_name(n0->dtype) << "|w" << dtype_name(ws[0].dtype) << "|t" << dtype_name(cos.dtype) << "|d" << dim << (full ? "|full" : "")
+     << "|nb" << nb << "|x" << count;
+  const std::string sig = sg.str();
+  wkf_kernel* k = kernel(sig, [&] {
+    return std::string(kPrelude) + define("WKF_H", n0->dtype == DType::F16) + define("WKF_WH", ws[0].dtype == DType::F16) + define("WKF_TH", cos.dtype == DType::F16) +
+           define("D", dim) + define("FULL", full) + define("NB", nb) + define("MEMBERS", count) + kNormRope;
+  });
+  const size_t e = dtype_size(n0->dtype);
+  for (size_t b0 = 0; b0 < batch; b0 += kMaxSequences) {
+    const size_t bn = std::min(batch - b0, kMaxSequences);
+    // Member[count], then cos, sin, seq, batch, heads, eps, positions[nb]: kernels/norm_rope.hip.inc
+    std::vector<unsigned char> block;
+    auto put = [&](const void* p, size_t bytes) { block.insert(block.end(), static_cast<const unsigned char*>(p), static_cast<const unsigned char*>(p) + bytes); };
+    for (size_t i = 0; i < count; i++) {
+      const Layout& l = xs[i].layout;
+      const size_t r = l.rank(), hn = nr_dim(members[i], 1);
+      struct {
+        const void *x, *y, *w;
+        uint64_t sb, sh, ss, yb;
+        uint32_t heads, pad;
+      } m = {first(xs[i]) + (r == 4 ? b0 * l.strides[0] * e : 0), first(outs[i]) + b0 * hn * seq * dim * e, first(ws[i]),
+             r == 4 ? l.strides[0] : 0, l.strides[r - 3], l.strides[r - 2], hn * seq * dim, uint32_t(hn), 0};
+      put(&m, sizeof(m));
+    }
+    struct {
+      const void *cos, *sin;
+      uint32_t seq, batch, heads;
+      float eps;
+    } t = {first(cos), first(sin), uint32_t(seq), uint32_t(bn), uint32_t(heads), args.eps};
+    put(&t, sizeof(t));
+    std::vector<uint32_t> pos(args.positions.begin() + b0, args.positions.begin() + b0 + bn);
+    pos.resize(nb);
+    put(pos.data(), nb * 4);
+    LaunchRecord r;
+    r.kind = "norm_rope";
+    r.signature = sig;
+    std::ostringstream d;
+    d << "batch=" << bn << " heads=" << heads << " seq=" << seq << " dim=" << dim << " tensors=" << count;
+    r.detail = d.str();
+    r.block[0] = 256;
+    r.grid[0] = grid_dim((bn * heads * seq + 3) / 4, "norm_rope");
+    record(std::move(r), k, block);
+  }
+  return outs;
+}
+
+// ---- the cache and its attention --------------------------------------------------------------------
+
+namespace {
+// the strides of a [sequences, heads, S, dim] tensor, or of one without the first dimension
+struct Strides4 {
+  uint64_t b, h, s;
+  explicit Strides4(const Layout& l) : b(l.rank() == 4 ? l.strides[0] : 0), h(l.strides[l.rank() - 3]), s(l.strides[l.rank() - 2]) {}
+};
+
+template <size_t NB>
+struct AppendArgs {
+  const void* in[2];
+  void *codes, *scales, *staged;
+  uint64_t sb[2], sh[2], ss[2];
+  uint32_t heads, cap, seqs, pad;
+  uint32_t len[NB], cnt[NB];
+};
+template <size_t NB>
+struct ValuesArgs {
+  void* out;
+  const void *codes, *scales;
+  uint32_t heads, cap, seqs, first, count, pad;
+  uint32_t len[NB];
+};
+template <size_t NB>
+struct AttendArgs {
+  const void* q;
+  void* out;
+  const void *codes, *scales;
+  uint64_t sb, sh, ss;
+  uint32_t heads, share, rows, seqs, cap, causal;
+  float scale;
+  uint32_t pad;
+  uint32_t len[NB], cnt[NB];
+};
+
+// `f` with the argument block of the cache's size class
+template <template <size_t> class A, typename F>
+void with_room(size_t nb, F&& f) {
+  if (nb == 8) {
+    A<8> a = {};
+    f(a);
+  } else if (nb == 64) {
+    A<64> a = {};
+    f(a);
+  } else {
+    A<kMaxSequences> a = {};
+    f(a);
+  }
+}
+}  // namespace
+
+void Resolver::append(KvCache& c, const NodeP& kn, const NodeP& vn, const std::vector<size_t>& counts) {
+  // what k and v take to compute is launched before the cache is looked at
+  std::vector<TensorData> in = resolve_roots({kn, vn});
+  for (TensorData& t : in)
+    if (t.layout.shape.back() > 1 && t.layout.strides.back() != 1) t = make_contiguous(t);
+  std::lock_guard<std::mutex> lock(c.mu);
+  size_t blocks = 0, total = 0;
+  for (size_t b = 0; b < c.seqs; b++) {
+    if (counts[b] > c.capacity - c.len[b])
+      invalid("kv_cache_append: sequence " + std::to_string(b) + " would have " + std::to_string(c.len[b] + counts[b]) + " tokens, the cache has room for " + std::to_string(c.capacity));
+    total += counts[b];
+    if (counts[b]) blocks = std::max(blocks, (c.len[b] + counts[b] - 1) / c.block - c.len[b] / c.block + 1);
+  }
+  if (!total) return;
+  const size_t nb = room_for(c.seqs);
+  const std::string sig = kv_signature("kv_append", c, kn->dtype, nb);
+  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + kv_defines(c, kn->dtype, nb) + kKvLayout + kKvAppend; });
+  with_room<AppendArgs>(nb, [&](auto& a) {
+    for (int i = 0; i < 2; i++) {
+      const Strides4 st(in[i].layout);
+      a.in[i] = first(in[i]);
+      a.sb[i] = st.b;
+      a.sh[i] = st.h;
+      a.ss[i] = st.s;
+    }
+    a.codes = ptr(c.codes);
+    a.scales = ptr(c.scales);
+    a.staged = ptr(c.staged);
+    a.heads = uint32_t(c.heads);
+    a.cap = uint32_t(c.cap);
+    a.seqs = uint32_t(c.seqs);
+    for (size_t b = 0; b < c.seqs; b++) {
+      a.len[b] = c.len[b];
+      a.cnt[b] = uint32_t(counts[b]) | uint32_t(c.slot[b]) << 31;
+    }
+    launch("kv_append", sig, "tokens=" + std::to_string(total), k, grid_dim(blocks, "kv_cache_append"), uint32_t(c.heads), uint32_t(2 * c.seqs), 256, a);
+  });
+  c.generation++;
+  for (size_t b = 0; b < c.seqs; b++) {
+    if (!counts[b]) continue;
+    const size_t end = c.len[b] + counts[b];
+    if ((end - 1) / c.block != c.len[b] / c.block) c.slot[b] ^= 1;  // the block that is open now was staged in the other slot
+    c.len[b] = uint32_t(end);
+  }
+}
+
+TensorData Resolver::run_cache_values(const NodeP& n) {
+  const CacheArgs& args = static_cast<const CacheArgs&>(*n->decode);
+  KvCache& c = *args.c;
+  std::lock_guard<std::mutex> lock(c.mu);
+  if (c.generation != args.generation) invalid("kv_cache_values: the cache has been appended to or reset since this tensor was recorded");
+  TensorData out = result_of(n.get());
+  if (!args.count) return out;
+  const size_t nb = room_for(c.seqs);
+  const std::string sig = kv_signature("kv_values", c, n->dtype, nb);
+  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + kv_defines(c, n->dtype, nb) + kKvLayout + kKvValues; });
+  with_room<ValuesArgs>(nb, [&](auto& a) {
+    a.out = first(out);
+    a.codes = ptr(c.codes);
+    a.scales = ptr(c.scales);
+    a.heads = uint32_t(c.heads);
+    a.cap = uint32_t(c.cap);
+    a.seqs = uint32_t(c.seqs);
+    a.first = uint32_t(args.first);
+    a.count = uint32_t(args.count);
+    std::copy(c.len.begin(), c.len.end(), a.len);
+    launch("kv_values", sig, "tokens=" + std::to_string(args.count), k, grid_dim((args.count + 15) / 16, "kv_cache_values"), uint32_t(c.heads), uint32_t(2 * c.seqs), 256, a);
+  });
+  return out;
+}
+
+TensorData Resolver::run_attend(const NodeP& n) {
+  const CacheArgs& args = static_cast<const CacheArgs&>(*n->decode);
+  KvCache& c = *args.c;
+  TensorData q = rows_dense(n->a);
+  std::lock_guard<std::mutex> lock(c.mu);
+  if (c.generation != args.generation) invalid("attend: the cache has been appended to or reset since this tensor was recorded");
+  TensorData out = result_of(n.get());
+  const size_t R = n->shape.size(), rows = n->shape[R - 2], heads = n->shape[R - 3];
+  if (!out.layout.numel()) return out;
+  const size_t nb = room_for(c.seqs);
+  const std::string sig = kv_signature("attend", c, n->dtype, nb);
+  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + kv_defines(c, n->dtype, nb) + kKvLayout + kAttend; });
+  with_room<AttendArgs>(nb, [&](auto& a) {
+    const Strides4 st(q.layout);
+    a.q = first(q);
+    a.out = first(out);
+    a.codes = ptr(c.codes);
+    a.scales = ptr(c.scales);
+    a.sb = st.b;
+    a.sh = st.h;
+    a.ss = st.s;
+    a.heads = uint32_t(c.heads);
+    a.share = uint32_t(heads / c.heads);
+    a.rows = uint32_t(rows);
+    a.seqs = uint32_t(c.seqs);
+    a.cap = uint32_t(c.cap);
+    a.causal = args.causal;
+    a.scale = args.scale;
+    std::copy(c.len.begin(), c.len.end(), a.len);
+    std::copy(args.counts.begin(), args.counts.end(), a.cnt);
+    std::ostringstream d;
+    d << "sequences=" << c.seqs << " heads=" << heads << "/" << c.heads << " rows=" << rows << " dim=" << c.dim;
+    launch("attend", sig, d.str(), k, grid_dim(rows, "attend"), uint32_t(heads), uint32_t(c.seqs), 256, a);
+  });
+  return out;
+}
+
+}  // namespace wkf

@@ -635,6 +635,10 @@ TensorData Resolver::resolve_uncached(const NodeP& n) {
     case NodeKind::MapLayout: return run_map_layout(n);
     case NodeKind::Resize: return run_resize(n);
     case NodeKind::SliceAssign: return run_slice_assign(n);
+    case NodeKind::MatMulQ4: return run_mat_mul_q4(n);
+    case NodeKind::NormRope: return run_norm_rope(n);
+    case NodeKind::CacheValues: return run_cache_values(n);
+    case NodeKind::Attend: return run_attend(n);
   }
   invalid("resolve: unknown node kind");
 }
@@ -662,6 +666,7 @@ TensorData Resolver::resolve_root(const NodeP& root) {
     }
     walk(n->a);
     walk(n->b);
+    for (const NodeP& m : n->more) walk(m);
   };
   // Under the reference rules nothing is shared: a node used twice is computed twice.
   if (st_.fusion == FusionMode::Tree) walk(root);
@@ -689,6 +694,7 @@ std::vector<TensorData> Resolver::resolve_roots(const std::vector<NodeP>& roots)
     }
     walk(n->a);
     walk(n->b);
+    for (const NodeP& m : n->more) walk(m);
   };
   if (st_.fusion == FusionMode::Tree) {
     for (const NodeP& r : roots) walk(r);
@@ -717,6 +723,7 @@ std::vector<TensorData> Resolver::resolve_roots(const std::vector<NodeP>& roots)
       if (try_parallel_reduces(g.second, &outs))
         for (size_t i = 0; i < g.second.size(); i++) materialized_[g.second[i].root] = outs[i];
     }
+    join_norm_ropes(roots);
   }
   std::vector<TensorData> out;
   for (const NodeP& r : roots) {
@@ -727,6 +734,62 @@ std::vector<TensorData> Resolver::resolve_roots(const std::vector<NodeP>& roots)
   materialized_.clear();
   sliced_.clear();
   return out;
+}
+
+// The outputs of wkf_tensor_materialize_into.  The decoder operators' kernels write a root's output tensor themselves
+// (result_of) unless its buffer is a leaf of the graph; every other root is computed as usual and copied.
+void Resolver::resolve_roots_into(const std::vector<NodeP>& roots, const std::vector<TensorData>& outs) {
+  std::set<const wkf_buffer*> leaves;
+  std::set<const Node*> seen;
+  std::function<void(const NodeP&)> walk = [&](const NodeP& n) {
+    if (!n || !seen.insert(n.get()).second) return;
+    if (n->kind == NodeKind::Tensor) leaves.insert(n->data.buffer.get());
+    walk(n->a);
+    walk(n->b);
+    for (const NodeP& m : n->more) walk(m);
+  };
+  for (const NodeP& r : roots) walk(r);
+  for (size_t i = 0; i < roots.size(); i++)
+    if (!leaves.count(outs[i].buffer.get())) results_.emplace(roots[i].get(), outs[i]);
+  std::vector<TensorData> got = resolve_roots(roots);
+  results_.clear();
+  for (size_t i = 0; i < roots.size(); i++) {
+    if (got[i].buffer.get() == outs[i].buffer.get() && got[i].layout == outs[i].layout) continue;
+    if (!got[i].layout.numel()) continue;
+    // an output that shares its buffer with the value of another root (a leaf that is a root itself, or a view of one)
+    // is overwritten here only after that value has been copied aside
+    for (size_t j = i + 1; j < roots.size(); j++)
+      if (got[j].buffer.get() == outs[i].buffer.get()) {
+        TensorData aside = alloc(got[j].layout.shape, got[j].dtype, false);
+        copy_map(got[j], aside);
+        got[j] = aside;
+      }
+    TensorData from = got[i];
+    if (from.buffer.get() == outs[i].buffer.get()) {  // a view of the output's own buffer in another order
+      TensorData aside = alloc(from.layout.shape, from.dtype, false);
+      copy_map(from, aside);
+      from = aside;
+    }
+    copy_map(from, outs[i]);
+  }
+}
+
+// A decoder operator's result: the caller's output tensor where there is one, else a new buffer.
+TensorData Resolver::result_of(const Node* n) {
+  auto it = results_.find(n);
+  if (it != results_.end()) return it->second;
+  return alloc(n->shape, n->dtype, false);
+}
+
+void Resolver::copy_map(const TensorData& from, const TensorData& to) {
+  Program p;
+  Instr in;
+  in.op = Op::Load;
+  in.dtype = from.dtype;
+  in.operand = 0;
+  p.ins.push_back(in);
+  p.result = 0;
+  launch_map(p, {from}, to, false);
 }
 
 // ---- row kernels -----------------------------------------------------------------------------
@@ -1496,14 +1559,7 @@ void Resolver::launch_map_tiled(MapSpec& spec, const Space& sp, const std::vecto
 TensorData Resolver::make_contiguous(const TensorData& td) {
   if (td.layout.is_contiguous()) return td;
   TensorData out = alloc(td.layout.shape, td.dtype, false);
-  Program p;
-  Instr in;
-  in.op = Op::Load;
-  in.dtype = td.dtype;
-  in.operand = 0;
-  p.ins.push_back(in);
-  p.result = 0;
-  launch_map(p, {td}, out, false);
+  copy_map(td, out);
   return out;
 }
 

@@ -91,6 +91,12 @@ class Resolver {
     bool out_taken = false, scratch_taken = false;
   };
   void set_noalloc(NoAlloc* na) { noalloc_ = na; }
+  // Several tensors in one pass, each into a dense tensor of the caller's (wkf_tensor_materialize_into).
+  void resolve_roots_into(const std::vector<NodeP>& roots, const std::vector<TensorData>& outs);
+  // wkf_kv_cache_append: materialises k and v and stores them.
+  void append(struct KvCache& c, const NodeP& k, const NodeP& v, const std::vector<size_t>& counts);
+  // wkf_q4_new: row-major codes, scales and zeros on the device -> the layout of the kernels.
+  void pack_q4(struct Q4& w, const TensorData& codes, const TensorData& scales, const TensorData& zeros);
   // whether any launch of this resolver was a team row kernel (whose result needs team_gave_up before it leaves)
   bool team_launched() const { return team_launched_; }
 
@@ -152,6 +158,32 @@ class Resolver {
   TensorData run_map_layout(const NodeP& n);
   TensorData run_resize(const NodeP& n);
   TensorData run_slice_assign(const NodeP& n);
+  // decoder operators (decode.cpp)
+  TensorData run_mat_mul_q4(const NodeP& n);
+  TensorData run_norm_rope(const NodeP& n);
+  TensorData run_cache_values(const NodeP& n);
+  TensorData run_attend(const NodeP& n);
+  // sibling norm_rope roots (the heads of q and of k) as one launch; leaves their values in materialized_
+  void join_norm_ropes(const std::vector<NodeP>& roots);
+  std::vector<TensorData> launch_norm_rope(const std::vector<const Node*>& members);
+  TensorData rows_dense(const NodeP& n);
+  TensorData result_of(const Node* n);
+  void copy_map(const TensorData& from, const TensorData& to);
+  template <typename A>
+  void launch(const char* kind, const std::string& sig, const std::string& detail, wkf_kernel* k, uint32_t gx, uint32_t gy, uint32_t gz,
+              uint32_t threads, const A& args) {
+    static_assert(sizeof(A) % 8 == 0, "the argument block is padded to a multiple of 8 bytes");
+    LaunchRecord r;
+    r.kind = kind;
+    r.signature = sig;
+    r.detail = detail;
+    r.grid[0] = gx;
+    r.grid[1] = gy;
+    r.grid[2] = gz;
+    r.block[0] = threads;
+    const unsigned char* p = reinterpret_cast<const unsigned char*>(&args);
+    record(std::move(r), k, std::vector<unsigned char>(p, p + sizeof(A)));
+  }
 
   // out[i] = prog(operands[i]) over out.layout.shape; every operand layout has that shape.
   // `more_prog[j]` (over the same operands) is stored to `more_out[j]` by the same kernel.
@@ -180,6 +212,7 @@ class Resolver {
   Settings st_;
   std::vector<LaunchRecord>* log_;
   std::set<const Node*> shared_;
+  std::map<const Node*, TensorData> results_;       // roots whose kernels write the caller's output tensor
   std::map<const Node*, TensorData> materialized_;  // nodes with several consumers, computed once per resolve
   std::map<std::tuple<const Node*, size_t, size_t, size_t>, NodeP> sliced_;  // slice_through results (and owners of its temporary nodes)
 };

@@ -9,19 +9,11 @@
 #include <sstream>
 #include <unordered_map>
 
-#include "graph.h"
+#include "tensor_api.h"
 
 using namespace wkf;
 
-// hip_ffi.cpp owns the thread-local error string; this hook lets the upper layers set it.
-void wkf_set_last_error_(const char* msg);
 void wkf_add_destroy_hook_(void (*fn)(wkf_device*));
-
-struct wkf_tensor {
-  wkf_device* dev;
-  NodeP node;
-  std::vector<LaunchRecord> launches;  // of the last materialize
-};
 
 struct wkf_slice {
   std::vector<unsigned char> bytes;
@@ -93,7 +85,9 @@ void forget_device(wkf_device* dev) {
   g_settings.erase(dev);
 }
 
-Settings settings_for(wkf_device* dev) {
+}  // namespace
+
+Settings wkf::settings_for(wkf_device* dev) {
   static const bool hooked = (wkf_add_destroy_hook_(&forget_device), true);
   (void)hooked;
   std::lock_guard<std::mutex> lock(g_settings_mu);
@@ -148,45 +142,7 @@ Settings settings_for(wkf_device* dev) {
   return it->second;
 }
 
-// Runs `f`, mapping exceptions to status codes + wkf_last_error().
-template <typename F>
-int guarded(F&& f) {
-  try {
-    f();
-    return WKF_OK;
-  } catch (const Error& e) {
-    wkf_set_last_error_(e.what());
-    return e.code;
-  } catch (const std::bad_alloc&) {
-    wkf_set_last_error_("host allocation failed");
-    return WKF_ERR_OOM;
-  } catch (const std::exception& e) {
-    wkf_set_last_error_(e.what());
-    return WKF_ERR_INVALID_ARG;
-  } catch (...) {
-    wkf_set_last_error_("unknown exception");
-    return WKF_ERR_INVALID_ARG;
-  }
-}
-
-wkf_tensor* wrap(wkf_device* dev, NodeP n) {
-  wkf_tensor* t = new wkf_tensor();
-  t->dev = dev;
-  t->node = std::move(n);
-  return t;
-}
-
-void need(const void* p, const char* what) {
-  if (!p) invalid(std::string(what) + ": null argument");
-}
-
-NodeP make(NodeKind k, DType dt, std::vector<size_t> shape) {
-  NodeP n = std::make_shared<Node>();
-  n->kind = k;
-  n->dtype = dt;
-  n->shape = std::move(shape);
-  return n;
-}
+namespace {
 
 // ---- node constructors (LazyTensorData::*, src/tensor.rs:179-284) -----------
 
@@ -925,6 +881,7 @@ std::string graph_dot(const NodeP& root) {
     if (n->kind != NodeKind::Tensor) {
       if (n->a) inputs.push_back(visit(n->a));
       if (n->b) inputs.push_back(visit(n->b));
+      for (const NodeP& m : n->more) inputs.push_back(visit(m));
     }
     const char* name = "tensor";
     switch (n->kind) {
@@ -936,6 +893,10 @@ std::string graph_dot(const NodeP& root) {
       case NodeKind::MapLayout: name = "slice"; break;
       case NodeKind::Resize: name = "resize"; break;
       case NodeKind::SliceAssign: name = "slice_assign"; break;
+      case NodeKind::MatMulQ4: name = "matmul_q4"; break;
+      case NodeKind::NormRope: name = "norm_rope"; break;
+      case NodeKind::CacheValues: name = "cache_values"; break;
+      case NodeKind::Attend: name = "attend"; break;
     }
     std::ostringstream id;
     id << '"' << name << " ([";
