@@ -23,8 +23,14 @@ const char* const kKvAppend =
 const char* const kKvValues =
 #include "kernels/kv_values.hip.inc"
     ;
-const char* const kAttend =
-#include "kernels/attend.hip.inc"
+const char* const kKvCodes =
+#include "kernels/kv_codes.hip.inc"
+    ;
+const char* const kAttendRows =
+#include "kernels/attend_rows.hip.inc"
+    ;
+const char* const kAttendJoin =
+#include "kernels/attend_join.hip.inc"
     ;
 const char* const kNormRope =
 #include "kernels/norm_rope.hip.inc"
@@ -244,10 +250,18 @@ struct AttendArgs {
   const void* q;
   void* out;
   const void *codes, *scales;
+  void *part, *stat;
   uint64_t sb, sh, ss;
   uint32_t heads, share, rows, seqs, cap, causal;
   float scale;
-  uint32_t pad;
+  uint32_t splits, span, tiles;
+  uint32_t len[NB], cnt[NB];
+};
+template <size_t NB>
+struct JoinArgs {
+  void* out;
+  const void *part, *stat;
+  uint32_t heads, share, rows, seqs, causal, splits, span, tiles;
   uint32_t len[NB], cnt[NB];
 };
 
@@ -347,30 +361,70 @@ TensorData Resolver::run_attend(const NodeP& n) {
   TensorData out = result_of(n.get());
   const size_t R = n->shape.size(), rows = n->shape[R - 2], heads = n->shape[R - 3];
   if (!out.layout.numel()) return out;
-  const size_t nb = room_for(c.seqs);
-  const std::string sig = kv_signature("attend", c, n->dtype, nb);
-  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + kv_defines(c, n->dtype, nb) + kKvLayout + kAttend; });
+  const size_t nb = room_for(c.seqs), share = heads / c.heads, tiles = (share * rows + 15) / 16;
+  // How many groups of 32 tokens a workgroup takes: enough workgroups to give every compute unit four, but a whole
+  // number of rounds of the four waves each.
+  size_t total = 0, longest = 0;
+  for (uint32_t n : c.len) {
+    total += (n + 31) / 32;
+    longest = std::max<size_t>(longest, (n + 31) / 32);
+  }
+  const size_t target = 1024;
+  size_t span = (total * c.heads * tiles + target - 1) / target;
+  span = std::max<size_t>(4, (span + 3) / 4 * 4);
+  const size_t splits = std::max<size_t>(1, (longest + span - 1) / span);
+  TensorData part, stat;
+  if (splits > 1) {
+    part = alloc({splits, c.seqs, c.heads, tiles, 16, c.dp}, DType::F32, false);
+    stat = alloc({splits, c.seqs, c.heads, tiles, 32}, DType::F32, false);
+  }
+  const std::string sig = kv_signature("attend_rows", c, n->dtype, nb);
+  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + kv_defines(c, n->dtype, nb) + kKvLayout + kKvCodes + kAttendRows; });
+  std::ostringstream d;
+  d << "sequences=" << c.seqs << " heads=" << heads << "/" << c.heads << " rows=" << rows << " dim=" << c.dim << " splits=" << splits;
   with_room<AttendArgs>(nb, [&](auto& a) {
     const Strides4 st(q.layout);
     a.q = first(q);
     a.out = first(out);
     a.codes = ptr(c.codes);
     a.scales = ptr(c.scales);
+    a.part = splits > 1 ? ptr(part.buffer) : nullptr;
+    a.stat = splits > 1 ? ptr(stat.buffer) : nullptr;
     a.sb = st.b;
     a.sh = st.h;
     a.ss = st.s;
     a.heads = uint32_t(c.heads);
-    a.share = uint32_t(heads / c.heads);
+    a.share = uint32_t(share);
     a.rows = uint32_t(rows);
     a.seqs = uint32_t(c.seqs);
     a.cap = uint32_t(c.cap);
     a.causal = args.causal;
     a.scale = args.scale;
+    a.splits = uint32_t(splits);
+    a.span = uint32_t(span);
+    a.tiles = uint32_t(tiles);
     std::copy(c.len.begin(), c.len.end(), a.len);
     std::copy(args.counts.begin(), args.counts.end(), a.cnt);
-    std::ostringstream d;
-    d << "sequences=" << c.seqs << " heads=" << heads << "/" << c.heads << " rows=" << rows << " dim=" << c.dim;
-    launch("attend", sig, d.str(), k, grid_dim(rows, "attend"), uint32_t(heads), uint32_t(c.seqs), 256, a);
+    launch("attend_rows", sig, d.str(), k, grid_dim(splits * tiles, "attend"), uint32_t(c.heads), uint32_t(c.seqs), 256, a);
+  });
+  if (splits == 1) return out;
+  const std::string jsig = kv_signature("attend_join", c, n->dtype, nb);
+  wkf_kernel* jk = kernel(jsig, [&] { return std::string(kPrelude) + kv_defines(c, n->dtype, nb) + kAttendJoin; });
+  with_room<JoinArgs>(nb, [&](auto& a) {
+    a.out = first(out);
+    a.part = ptr(part.buffer);
+    a.stat = ptr(stat.buffer);
+    a.heads = uint32_t(c.heads);
+    a.share = uint32_t(share);
+    a.rows = uint32_t(rows);
+    a.seqs = uint32_t(c.seqs);
+    a.causal = args.causal;
+    a.splits = uint32_t(splits);
+    a.span = uint32_t(span);
+    a.tiles = uint32_t(tiles);
+    std::copy(c.len.begin(), c.len.end(), a.len);
+    std::copy(args.counts.begin(), args.counts.end(), a.cnt);
+    launch("attend_join", jsig, d.str(), jk, grid_dim((share * rows + 3) / 4, "attend"), uint32_t(c.heads), uint32_t(c.seqs), 256, a);
   });
   return out;
 }

@@ -36,7 +36,7 @@ struct Q4 {
 struct KvCache {
   wkf_device* dev = nullptr;
   size_t seqs = 0, heads = 0, dim = 0, dp = 0, block = 0;
-  size_t capacity = 0, cap = 0;  // tokens of a sequence: what was asked for, and rounded up to whole blocks
+  size_t capacity = 0, cap = 0;  // tokens of a sequence: what was asked for, and rounded up to whole blocks and to 64
   BufRef codes, scales, staged;
   std::mutex mu;  // lengths, slots and generation; held while a launch that goes by them is put on the stream
   std::vector<uint32_t> len;

@@ -1,6 +1,7 @@
 // The C entry points of include/wkf_decode.h.
 #include "wkf_decode.h"
 
+#include <algorithm>
 #include <cmath>
 #include <cstring>
 
@@ -263,7 +264,8 @@ int wkf_kv_cache_create(wkf_device* dev, size_t sequences, size_t kv_heads, size
     c->dim = head_dim;
     c->dp = (head_dim + 63) / 64 * 64;
     c->block = block;
-    c->cap = (capacity + block - 1) / block * block;
+    const size_t whole = std::max<size_t>(block, 64);
+    c->cap = (capacity + whole - 1) / whole * whole;
     const size_t rows = 2 * sequences * kv_heads;
     c->codes = buffer(dev, times(times(rows, c->cap, who), c->dp, who));
     c->scales = buffer(dev, times(rows, c->cap / block, who) * 4);
