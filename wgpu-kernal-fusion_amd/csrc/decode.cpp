@@ -38,6 +38,9 @@ const char* const kNormRope =
 const char* const kQ4Pack =
 #include "kernels/q4_pack.hip.inc"
     ;
+const char* const kQ4Dense =
+#include "kernels/q4_dense.hip.inc"
+    ;
 const char* const kQ4MatMul =
 #include "kernels/q4_mat_mul.hip.inc"
     ;
@@ -94,12 +97,25 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
   TensorData x = resolve(n->a);
   if (x.layout.strides != Layout::contiguous_strides(x.layout.shape)) x = make_contiguous(x);
   TensorData out = result_of(n.get());
-  const size_t M = x.layout.numel() / w.k, N = w.n;
+  const size_t M = x.layout.numel() / w.k, N = w.n, Kp = (w.k + 7) / 8 * 8;
   if (!M) return out;
   if (M > 0xfffffull) throw Error(WKF_ERR_UNSUPPORTED, "mat_mul_q4: more than 2^20 rows");
-  const bool z = bool(w.zeros), h = x.dtype == DType::F16, sh = w.scale_dtype == DType::F16;
-  const std::string sig = std::string("q4_mat_mul|gfx950|") + dtype_name(x.dtype) + "|s" + dtype_name(w.scale_dtype) + (z ? "|zeros" : "");
-  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + define("WKF_H", h) + define("WKF_SH", sh) + define("WKF_Z", z) + kQ4MatMul; });
+  // Many f16 rows: the weights are written out once and the product is mat_mul's.
+  if (x.dtype == DType::F16 && M > 64 && N >= 16 && M * N * Kp >= (size_t(1) << 18)) return mat_mul_q4_dense(w, x, out, M);
+  const bool z = bool(w.zeros);
+  // the k = 32 steps of a tile that surely share a group, and the group in units of so many
+  const size_t step = w.group % 128 == 0 ? 4 : w.group % 64 == 0 ? 2 : 1, units = w.group / (32 * step);
+  int shift = -1;
+  for (int i = 0; i < 32; i++)
+    if (units == size_t(1) << i) shift = i;
+  const size_t mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
+  std::ostringstream sg;
+  sg << "q4_mat_mul|gfx950|" << dtype_name(x.dtype) << "|s" << dtype_name(w.scale_dtype) << (z ? "|zeros" : "") << "|mt" << mt << "|step" << step << "|shift" << shift;
+  const std::string sig = sg.str();
+  wkf_kernel* k = kernel(sig, [&] {
+    return std::string(kPrelude) + define("WKF_H", x.dtype == DType::F16) + define("WKF_SH", w.scale_dtype == DType::F16) + define("WKF_Z", z) + define("MT", mt) +
+           define("STEP", step) + "#define SHIFT " + std::to_string(shift) + "\n" + kQ4MatMul;
+  });
   struct {
     const void *x, *codes, *scales, *zeros;
     void* y;
@@ -108,7 +124,59 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
          uint32_t(M), uint32_t(N), uint32_t(w.k), uint32_t(w.group), uint32_t(w.groups), uint32_t(w.tiles_k())};
   std::ostringstream d;
   d << "m=" << M << " n=" << N << " k=" << w.k << " group=" << w.group;
-  launch("q4_mat_mul", sig, d.str(), k, uint32_t(w.tiles_n()), uint32_t((M + 15) / 16), 1, 256, a);
+  launch("q4_mat_mul", sig, d.str(), k, uint32_t(w.tiles_n()), uint32_t((M + 16 * mt - 1) / (16 * mt)), 1, 512, a);
+  return out;
+}
+
+TensorData Resolver::mat_mul_q4_dense(const Q4& w, const TensorData& x_in, const TensorData& out, size_t M) {
+  const size_t N = w.n, Kp = (w.k + 7) / 8 * 8;
+  const bool z = bool(w.zeros), h = x_in.dtype == DType::F16;
+  // rows of x that start on 16 bytes: what mat_mul would otherwise see to by itself
+  TensorData x = x_in;
+  x.layout.shape = {M, w.k};
+  x.layout.strides = {w.k, 1};
+  if (Kp != w.k) {
+    TensorData padded = alloc({M, Kp}, x.dtype, true), corner = padded;
+    corner.layout.shape = {M, w.k};
+    copy_map(x, corner);
+    x = padded;
+  }
+  TensorData wt = alloc({N, Kp}, x.dtype, false);
+  const std::string sig = std::string("q4_dense|gfx950|") + dtype_name(x.dtype) + "|s" + dtype_name(w.scale_dtype) + (z ? "|zeros" : "");
+  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + define("WKF_H", h) + define("WKF_SH", w.scale_dtype == DType::F16) + define("WKF_Z", z) + kQ4Dense; });
+  struct {
+    const void *codes, *scales, *zeros;
+    void* out;
+    uint32_t n, k, stride, group, groups, tiles_k;
+  } a = {ptr(w.codes), ptr(w.scales), z ? ptr(w.zeros) : nullptr, ptr(wt.buffer), uint32_t(N), uint32_t(w.k), uint32_t(Kp), uint32_t(w.group), uint32_t(w.groups), uint32_t(w.tiles_k())};
+  if (w.tiles_n() > 65535) throw Error(WKF_ERR_UNSUPPORTED, "mat_mul_q4: more than 2^20 columns");
+  std::ostringstream d;
+  d << "n=" << N << " k=" << w.k << " group=" << w.group;
+  launch("q4_dense", sig, d.str(), k, uint32_t((w.tiles_k() + 3) / 4), uint32_t(w.tiles_n()), 1, 256, a);
+  auto leaf = [&](const TensorData& t) {
+    NodeP n = std::make_shared<Node>();
+    n->kind = NodeKind::Tensor;
+    n->dtype = t.dtype;
+    n->shape = t.layout.shape;
+    n->data = t;
+    return n;
+  };
+  TensorData b = wt;  // [K, N] as the transpose of the dense [N, K]
+  std::swap(b.layout.shape[0], b.layout.shape[1]);
+  std::swap(b.layout.strides[0], b.layout.strides[1]);
+  NodeP mm = std::make_shared<Node>();
+  mm->kind = NodeKind::MatMul;
+  mm->dtype = x.dtype;
+  mm->shape = {M, N};
+  mm->a = leaf(x);
+  mm->b = leaf(b);
+  TensorData flat = out;
+  flat.layout = Layout::contiguous({M, N});
+  flat.layout.offset = out.layout.offset;
+  if (st_.fusion == FusionMode::Tree) mat_mul_out_ = &flat;
+  TensorData got = run_matmul(mm);
+  mat_mul_out_ = nullptr;
+  if (got.buffer.get() != flat.buffer.get()) copy_map(got, flat);
   return out;
 }
 

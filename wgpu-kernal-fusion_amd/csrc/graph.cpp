@@ -516,6 +516,11 @@ bool Resolver::try_map_table(const Program& prog, const std::vector<TensorData>&
 }
 
 TensorData Resolver::alloc(const std::vector<size_t>& shape, DType dt, bool zero, bool result) {
+  if (mat_mul_out_ && !zero && shape == mat_mul_out_->layout.shape && dt == mat_mul_out_->dtype) {
+    const TensorData out = *mat_mul_out_;
+    mat_mul_out_ = nullptr;
+    return out;
+  }
   TensorData td;
   td.device = dev_;
   td.layout = Layout::contiguous(shape);

@@ -160,6 +160,7 @@ class Resolver {
   TensorData run_slice_assign(const NodeP& n);
   // decoder operators (decode.cpp)
   TensorData run_mat_mul_q4(const NodeP& n);
+  TensorData mat_mul_q4_dense(const struct Q4& w, const TensorData& x, const TensorData& out, size_t rows);
   TensorData run_norm_rope(const NodeP& n);
   TensorData run_cache_values(const NodeP& n);
   TensorData run_attend(const NodeP& n);
@@ -211,6 +212,9 @@ class Resolver {
   bool team_launched_ = false;
   Settings st_;
   std::vector<LaunchRecord>* log_;
+  // where run_matmul leaves its product, taken by the one allocation of its shape and dtype (mat_mul_q4_dense sees to it
+  // that no temporary has both); null: a new buffer
+  const TensorData* mat_mul_out_ = nullptr;
   std::set<const Node*> shared_;
   std::map<const Node*, TensorData> results_;       // roots whose kernels write the caller's output tensor
   std::map<const Node*, TensorData> materialized_;  // nodes with several consumers, computed once per resolve
