@@ -29,9 +29,6 @@ const char* const kKvCodes =
 const char* const kAttendRows =
 #include "kernels/attend_rows.hip.inc"
     ;
-const char* const kAttendJoin =
-#include "kernels/attend_join.hip.inc"
-    ;
 const char* const kNormRope =
 #include "kernels/norm_rope.hip.inc"
     ;
@@ -318,21 +315,13 @@ struct AttendArgs {
   const void* q;
   void* out;
   const void *codes, *scales;
-  void *part, *stat;
+  void *part, *stat, *done;
   uint64_t sb, sh, ss;
   uint32_t heads, share, rows, seqs, cap, causal;
   float scale;
   uint32_t splits, span, tiles;
   uint32_t len[NB], cnt[NB];
 };
-template <size_t NB>
-struct JoinArgs {
-  void* out;
-  const void *part, *stat;
-  uint32_t heads, share, rows, seqs, causal, splits, span, tiles;
-  uint32_t len[NB], cnt[NB];
-};
-
 // `f` with the argument block of the cache's size class
 template <template <size_t> class A, typename F>
 void with_room(size_t nb, F&& f) {
@@ -430,24 +419,33 @@ TensorData Resolver::run_attend(const NodeP& n) {
   const size_t R = n->shape.size(), rows = n->shape[R - 2], heads = n->shape[R - 3];
   if (!out.layout.numel()) return out;
   const size_t nb = room_for(c.seqs), share = heads / c.heads, tiles = (share * rows + 15) / 16;
-  // How many groups of 32 tokens a workgroup takes: enough workgroups to give every compute unit four, but a whole
-  // number of rounds of the four waves each.
+  // How many groups of 32 tokens a workgroup takes.  One workgroup for each compute unit is enough to read at the memory's
+  // rate (16 sequences of 8000 tokens, 32 key heads: 136 us with 256 workgroups, 152 with 1024); where there are fewer
+  // sequences and heads than that, each is split, but joining s parts costs about as much as reading s groups, so no
+  // finer than its square root (one sequence, 8 key heads: 4000 tokens 16.6 us in 32 parts, 11.7 in 11; 16000 tokens 21.4 us
+  // in 32 parts, 19.3 in 16).  Up to 16 groups stay whole: the join alone takes 3 us.
   size_t total = 0, longest = 0;
   for (uint32_t n : c.len) {
     total += (n + 31) / 32;
     longest = std::max<size_t>(longest, (n + 31) / 32);
   }
-  const size_t target = 1024;
+  constexpr size_t waves = 4, ahead = 2, target = 256;
   size_t span = (total * c.heads * tiles + target - 1) / target;
-  span = std::max<size_t>(4, (span + 3) / 4 * 4);
+  span = std::max(span, longest <= 16 ? longest : size_t(std::ceil(std::sqrt(double(longest)))));
+  span = std::max(waves, (span + waves - 1) / waves * waves);
   const size_t splits = std::max<size_t>(1, (longest + span - 1) / span);
   TensorData part, stat;
   if (splits > 1) {
     part = alloc({splits, c.seqs, c.heads, tiles, 16, c.dp}, DType::F32, false);
     stat = alloc({splits, c.seqs, c.heads, tiles, 32}, DType::F32, false);
+    const size_t counters = c.seqs * c.heads * tiles;
+    if (counters > c.counters) {  // zeros, and every launch leaves zeros
+      c.done = alloc({counters}, DType::F32, true).buffer;
+      c.counters = counters;
+    }
   }
-  const std::string sig = kv_signature("attend_rows", c, n->dtype, nb);
-  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + kv_defines(c, n->dtype, nb) + kKvLayout + kKvCodes + kAttendRows; });
+  const std::string sig = kv_signature("attend_rows", c, n->dtype, nb) + "|w" + std::to_string(waves);
+  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + define("W", waves) + define("AHEAD", ahead) + kv_defines(c, n->dtype, nb) + kKvLayout + kKvCodes + kAttendRows; });
   std::ostringstream d;
   d << "sequences=" << c.seqs << " heads=" << heads << "/" << c.heads << " rows=" << rows << " dim=" << c.dim << " splits=" << splits;
   with_room<AttendArgs>(nb, [&](auto& a) {
@@ -458,6 +456,7 @@ TensorData Resolver::run_attend(const NodeP& n) {
     a.scales = ptr(c.scales);
     a.part = splits > 1 ? ptr(part.buffer) : nullptr;
     a.stat = splits > 1 ? ptr(stat.buffer) : nullptr;
+    a.done = splits > 1 ? ptr(c.done) : nullptr;
     a.sb = st.b;
     a.sh = st.h;
     a.ss = st.s;
@@ -473,26 +472,7 @@ TensorData Resolver::run_attend(const NodeP& n) {
     a.tiles = uint32_t(tiles);
     std::copy(c.len.begin(), c.len.end(), a.len);
     std::copy(args.counts.begin(), args.counts.end(), a.cnt);
-    launch("attend_rows", sig, d.str(), k, grid_dim(splits * tiles, "attend"), uint32_t(c.heads), uint32_t(c.seqs), 256, a);
-  });
-  if (splits == 1) return out;
-  const std::string jsig = kv_signature("attend_join", c, n->dtype, nb);
-  wkf_kernel* jk = kernel(jsig, [&] { return std::string(kPrelude) + kv_defines(c, n->dtype, nb) + kAttendJoin; });
-  with_room<JoinArgs>(nb, [&](auto& a) {
-    a.out = first(out);
-    a.part = ptr(part.buffer);
-    a.stat = ptr(stat.buffer);
-    a.heads = uint32_t(c.heads);
-    a.share = uint32_t(share);
-    a.rows = uint32_t(rows);
-    a.seqs = uint32_t(c.seqs);
-    a.causal = args.causal;
-    a.splits = uint32_t(splits);
-    a.span = uint32_t(span);
-    a.tiles = uint32_t(tiles);
-    std::copy(c.len.begin(), c.len.end(), a.len);
-    std::copy(args.counts.begin(), args.counts.end(), a.cnt);
-    launch("attend_join", jsig, d.str(), jk, grid_dim((share * rows + 3) / 4, "attend"), uint32_t(c.heads), uint32_t(c.seqs), 256, a);
+    launch("attend_rows", sig, d.str(), k, grid_dim(splits * tiles, "attend"), uint32_t(c.heads), uint32_t(c.seqs), uint32_t(64 * waves), a);
   });
   return out;
 }
