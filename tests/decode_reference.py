@@ -126,3 +126,11 @@ def attend(q, k, v, scale, causal, length, count):
                 d = (dim + 4) * U32 * size.max() + 4 * U32 * max(1.0, np.abs(x).max())
                 slack[h, s] = (2 * d + (n + 16) * U32) * (p @ np.abs(vv)) / total * 2
     return out, slack
+
+
+def f16_weights_slack(q, k, v, scale, causal, length, count):
+    """What rounding each softmax weight to f16, before it meets the values, may add: U16 of every term, and for weights so
+    small that they are subnormal at least 2^-37 of the largest (a kernel gives its largest weight 2^12 or more, the step of
+    f16 subnormals is 2^-24, half of it 2^-25) times the largest value, for each token."""
+    a, _ = attend(q, k, np.abs(v), scale, causal, length, count)
+    return U16 * a + length * 2.0 ** -37 * (np.abs(v).max() if v.size else 0.0)

@@ -29,6 +29,9 @@ const char* const kKvCodes =
 const char* const kAttendRows =
 #include "kernels/attend_rows.hip.inc"
     ;
+const char* const kAttendPrompt =
+#include "kernels/attend_prompt.hip.inc"
+    ;
 const char* const kNormRope =
 #include "kernels/norm_rope.hip.inc"
     ;
@@ -322,6 +325,18 @@ struct AttendArgs {
   uint32_t splits, span, tiles;
   uint32_t len[NB], cnt[NB];
 };
+template <size_t NB>
+struct PromptArgs {
+  const void* q;
+  void* out;
+  const void *codes, *scales;
+  uint64_t sb, sh, ss;
+  uint32_t heads, share, rows, seqs, cap, causal;
+  float scale;
+  uint32_t tiles;
+  uint32_t len[NB], cnt[NB];
+};
+
 // `f` with the argument block of the cache's size class
 template <template <size_t> class A, typename F>
 void with_room(size_t nb, F&& f) {
@@ -419,6 +434,38 @@ TensorData Resolver::run_attend(const NodeP& n) {
   const size_t R = n->shape.size(), rows = n->shape[R - 2], heads = n->shape[R - 3];
   if (!out.layout.numel()) return out;
   const size_t nb = room_for(c.seqs), share = heads / c.heads, tiles = (share * rows + 15) / 16;
+  // Rows enough to give every compute unit a tile of 128: the kernel that spreads the codes in the LDS for all of them.
+  const size_t big = (share * rows + 127) / 128;
+  size_t bigmin = 128;
+  if (const char* e = getenv("WKF_X_B")) bigmin = atoi(e);
+  if (share * rows > 64 && big * c.heads * c.seqs >= bigmin) {
+    const std::string psig = kv_signature("attend_prompt", c, n->dtype, nb);
+    wkf_kernel* pk = kernel(psig, [&] { return std::string(kPrelude) + kv_defines(c, n->dtype, nb) + kKvLayout + kKvCodes + kAttendPrompt; });
+    with_room<PromptArgs>(nb, [&](auto& a) {
+      const Strides4 st(q.layout);
+      a.q = first(q);
+      a.out = first(out);
+      a.codes = ptr(c.codes);
+      a.scales = ptr(c.scales);
+      a.sb = st.b;
+      a.sh = st.h;
+      a.ss = st.s;
+      a.heads = uint32_t(c.heads);
+      a.share = uint32_t(share);
+      a.rows = uint32_t(rows);
+      a.seqs = uint32_t(c.seqs);
+      a.cap = uint32_t(c.cap);
+      a.causal = args.causal;
+      a.scale = args.scale;
+      a.tiles = uint32_t(big);
+      std::copy(c.len.begin(), c.len.end(), a.len);
+      std::copy(args.counts.begin(), args.counts.end(), a.cnt);
+      std::ostringstream d;
+      d << "sequences=" << c.seqs << " heads=" << heads << "/" << c.heads << " rows=" << rows << " dim=" << c.dim << " tiles of 128 rows";
+      launch("attend_prompt", psig, d.str(), pk, grid_dim(big * c.heads * c.seqs, "attend"), 1, 1, 256, a);
+    });
+    return out;
+  }
   // How many groups of 32 tokens a workgroup takes.  One workgroup for each compute unit is enough to read at the memory's
   // rate (16 sequences of 8000 tokens, 32 key heads: 136 us with 256 workgroups, 152 with 1024); where there are fewer
   // sequences and heads than that, each is split, but joining s parts costs about as much as reading s groups, so no
