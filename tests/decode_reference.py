@@ -108,23 +108,22 @@ def attend(q, k, v, scale, causal, length, count):
     heads, rows, dim = q.shape
     out, slack = np.zeros(q.shape), np.zeros(q.shape)
     share = heads // max(1, k.shape[0])
-    for h in range(heads):
-        for s in range(count):
-            n = length - count + s + 1 if causal else length
-            if n <= 0:
-                continue
-            kk, vv = k[h // share, :n], v[h // share, :n]
-            with np.errstate(invalid="ignore", over="ignore"):
-                x = kk @ q[h, s] * scale
-                size = np.abs(kk) @ np.abs(q[h, s]) * scale
-                p = np.exp(x - x.max())
-                total = p.sum()
-                out[h, s] = p @ vv / total
-                # a score: dim + 4 roundings of partial sums no larger than `size`, and the rounding of the exponent;
-                # a weight: that, twice (the row's largest score too), its own rounding and two of the exponential; sums of n
-                # weights and n products
-                d = (dim + 4) * U32 * size.max() + 4 * U32 * max(1.0, np.abs(x).max())
-                slack[h, s] = (2 * d + (n + 16) * U32) * (p @ np.abs(vv)) / total * 2
+    last = np.minimum(np.arange(count) + (length - count + 1 if causal else length), length)  # tokens a row sees
+    seen = np.arange(length)[None, :] < last[:, None]
+    for h in range(heads if count and length else 0):
+        kk, vv = k[h // share], v[h // share]
+        with np.errstate(invalid="ignore", over="ignore"):
+            x = np.where(seen, q[h, :count] @ kk.T * scale, -np.inf)
+            size = np.where(seen, np.abs(q[h, :count]) @ np.abs(kk).T * scale, 0)
+            p = np.where(seen, np.exp(x - x.max(1, keepdims=True)), 0)
+            total = p.sum(1, keepdims=True)
+            out[h, :count] = p @ vv / total
+            # a score: dim + 4 roundings of partial sums no larger than `size`, and the rounding of the exponent; a weight: that,
+            # twice (the row's largest score too), its own rounding and two of the exponential; sums of n weights and n products.
+            # What lies below 2^-126 of the largest weight is below f32's normals, and may count as zero: so may the parts
+            # of a weight that is taken in three, so 3 2^-126 times the largest value, for each token.
+            d = (dim + 4) * U32 * size.max(1) + 4 * U32 * np.maximum(1.0, np.abs(np.where(seen, x, 0)).max(1))
+            slack[h, :count] = (2 * d + (last + 16) * U32)[:, None] * (p @ np.abs(vv)) / total * 2 + (3 * 2.0 ** -126 * last * np.abs(vv).max())[:, None]
     return out, slack
 
 

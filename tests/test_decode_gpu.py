@@ -334,6 +334,27 @@ def test_attend(gpu, case, dtype):
     check_attend(gpu, dtype, lengths, heads, kv, dim, block, rows)
 
 
+# enough tiles of 128 rows for every compute unit
+PROMPT_CASES = [([150, 0, 129, 200], 32, 32, 64, 64, 129), ([100, 37, 300, 1, 128, 0], 48, 16, 72, 32, 100), ([141, 140, 0, 270, 64, 33], 32, 16, 128, 128, 140),
+                ([70, 90, 0, 5, 65, 64, 71, 200], 32, 32, 200, 32, 70), ([260] * 4, 32, 32, 128, 64, 256), ([400, 260], 64, 64, 16, 32, 200)]
+
+
+@DTYPES
+@pytest.mark.parametrize("case", PROMPT_CASES, ids=str)
+def test_attend_with_many_rows(gpu, case, dtype):
+    lengths, heads, kv, dim, block, rows = case
+    check_attend(gpu, dtype, lengths, heads, kv, dim, block, rows)
+
+
+@DTYPES
+def test_attend_with_many_rows_in_other_ways(gpu, dtype):
+    check_attend(gpu, dtype, [150, 0, 190, 65], 64, 64, 64, 32, 70, causal=False)
+    check_attend(gpu, dtype, [150, 0, 190, 65], 64, 64, 64, 32, 70, counts=[70, 0, 33, 1])
+    check_attend(gpu, dtype, [150, 0, 190, 65], 128, 64, 64, 64, 100, counts=[64, 0, 100, 65], causal=False)
+    for scale in (0.0, 4.0):
+        check_attend(gpu, dtype, [150, 10, 190, 65], 64, 64, 64, 64, 70, scale=scale)
+
+
 @DTYPES
 @pytest.mark.parametrize("rows", [1, 3, 30, 70])
 def test_attend_to_the_whole_sequence(gpu, rows, dtype):
@@ -369,41 +390,41 @@ def test_attend_takes_views_of_q(gpu, dtype):
 
 
 @DTYPES
-@pytest.mark.parametrize("rows", [4, 40])
-def test_attend_keeps_nan_and_infinities_of_q_in_their_rows(gpu, rows, dtype):
+@pytest.mark.parametrize("rows,kv", [(4, 1), (40, 1), (70, 256)])
+def test_attend_keeps_nan_and_infinities_of_q_in_their_rows(gpu, rows, kv, dtype):
     rng = rng_of(42, rows)
-    cache, held, _ = filled(gpu, rng, dtype, [100], 1, 64, 32)
-    q = rng.standard_normal((2, rows, 64)).astype(dtype)
+    cache, held, _ = filled(gpu, rng, dtype, [100], kv, 64, 32)
+    q = rng.standard_normal((2 * kv, rows, 64)).astype(dtype)
     clean = computed(leaf(gpu, q).attend(cache))
     q[0, 1, 5], q[1, 2, 0] = np.nan, np.inf
     got = computed(leaf(gpu, q).attend(cache))
     assert np.all(np.isnan(got[0, 1])) and np.all(np.isnan(got[1, 2]))
-    rest = np.ones((2, rows), bool)
+    rest = np.ones((2 * kv, rows), bool)
     rest[0, 1] = rest[1, 2] = False
     assert np.array_equal(got[rest], clean[rest])
 
 
 @DTYPES
-@pytest.mark.parametrize("rows", [1, 60])
-def test_attend_over_zero_blocks_and_what_lies_behind_the_end(gpu, rows, dtype):
+@pytest.mark.parametrize("rows,kv", [(1, 2), (60, 2), (70, 256)])
+def test_attend_over_zero_blocks_and_what_lies_behind_the_end(gpu, rows, kv, dtype):
     """Blocks of zeros (scale 0) among others; infinities and NaN in tokens that a reset has forgotten."""
     w, rng = load_package(), rng_of(43, rows)
-    k, v = (rng.standard_normal((1, 2, 160, 64)).astype(dtype) for _ in range(2))
+    k, v = (rng.standard_normal((1, kv, 160, 64)).astype(dtype) for _ in range(2))
     v[:, :, 32:64] = 0
     k[:, :, 64:96] = 0
     v[:, 1] = 0  # a head without any values
-    cache = w.KvCache(gpu, 1, 2, 64, 320, 32)
-    cache.append(leaf(gpu, np.full((1, 2, 320, 64), np.inf, dtype)), leaf(gpu, np.full((1, 2, 320, 64), np.nan, dtype)))
+    cache = w.KvCache(gpu, 1, kv, 64, 320, 32)
+    cache.append(leaf(gpu, np.full((1, kv, 320, 64), np.inf, dtype)), leaf(gpu, np.full((1, kv, 320, 64), np.nan, dtype)))
     cache.reset()
     cache.append(leaf(gpu, k), leaf(gpu, v))
-    held = [np.stack([ref.values(x[0, h], 32) for h in range(2)]) for x in (k, v)]
-    q = rng.standard_normal((1, 4, rows, 64)).astype(dtype)
+    held = [np.stack([ref.values(x[0, h], 32) for h in range(kv)]) for x in (k, v)]
+    q = rng.standard_normal((1, 2 * kv, rows, 64)).astype(dtype)
     got = computed(leaf(gpu, q).attend(cache))
     want, slack = ref.attend(q[0], *held, 0.125, True, 160, rows)
     if dtype == F16:
         slack = slack + ref.f16_weights_slack(q[0], *held, 0.125, True, 160, rows)
     ref.close(got[0], want, dtype, slack)
-    assert np.all(got[0, 2:] == 0)
+    assert np.all(got[0, 2:4] == 0)
 
 
 def test_attend_of_an_empty_cache_and_of_no_rows(gpu):
@@ -417,9 +438,9 @@ def test_attend_of_an_empty_cache_and_of_no_rows(gpu):
 
 def test_attend_gives_the_same_bits_every_time(gpu):
     rng = rng_of(44)
-    cache, _, _ = filled(gpu, rng, F16, [5000, 1200], 2, 128, 64)
-    for rows in (1, 64):
-        t = leaf(gpu, rng.standard_normal((2, 8, rows, 128)).astype(F16)).attend(cache)
+    for kv, lengths, rows in ((2, [5000, 1200], 1), (2, [5000, 1200], 64), (64, [300, 200], 200)):
+        cache, _, _ = filled(gpu, rng, F16, lengths, kv, 128, 64)
+        t = leaf(gpu, rng.standard_normal((2, 4 * kv, rows, 128)).astype(F16)).attend(cache)
         first = computed(t)
         for _ in range(3):
             assert np.array_equal(computed(t), first)

@@ -434,11 +434,11 @@ TensorData Resolver::run_attend(const NodeP& n) {
   const size_t R = n->shape.size(), rows = n->shape[R - 2], heads = n->shape[R - 3];
   if (!out.layout.numel()) return out;
   const size_t nb = room_for(c.seqs), share = heads / c.heads, tiles = (share * rows + 15) / 16;
-  // Rows enough to give every compute unit a tile of 128: the kernel that spreads the codes in the LDS for all of them.
+  // Rows enough to give every compute unit a tile of 128: the kernel that spreads the codes in the LDS for all of them
+  // (2048 new tokens after 2048, 32/8 heads: 512 tiles, 133 us against 276 in tiles of 16 rows).  With fewer tiles the cache has
+  // to be split over workgroups, which the kernel for tiles of 16 rows does (512 new tokens after 3584: 101 us against 89).
   const size_t big = (share * rows + 127) / 128;
-  size_t bigmin = 128;
-  if (const char* e = getenv("WKF_X_B")) bigmin = atoi(e);
-  if (share * rows > 64 && big * c.heads * c.seqs >= bigmin) {
+  if (share * rows > 64 && big * c.heads * c.seqs >= 256) {
     const std::string psig = kv_signature("attend_prompt", c, n->dtype, nb);
     wkf_kernel* pk = kernel(psig, [&] { return std::string(kPrelude) + kv_defines(c, n->dtype, nb) + kKvLayout + kKvCodes + kAttendPrompt; });
     with_room<PromptArgs>(nb, [&](auto& a) {
