@@ -74,8 +74,14 @@ Q4_CASES = [  # m, k, n, group, zeros, scale dtype
     (1, 32, 16, 32, False, F16), (1, 1, 1, 32, True, F16), (3, 37, 5, 32, True, F32), (1, 4096, 64, 128, False, F16),
     (2, 130, 17, 64, True, F16), (16, 256, 48, 96, False, F32), (17, 384, 33, 128, True, F16), (5, 1000, 100, 1024, False, F16),
     (40, 512, 80, 64, True, F16), (65, 640, 130, 32, False, F16), (128, 256, 256, 128, True, F16), (300, 200, 264, 64, True, F32),
-    (513, 1024, 272, 128, False, F16),
+    (513, 1024, 272, 128, False, F16), (24, 200, 40, 64, False, F16), (20, 136, 4200, 32, True, F16), (33, 264, 48, 128, True, F32), (600, 96, 2000, 32, True, F16),
+    (300, 160, 2000, 64, False, F16), (1100, 130, 2000, 128, True, F16), (800, 203, 144, 96, True, F32), (768, 64, 64, 32, False, F16), (7, 1290, 1037, 64, True, F16),
 ]
+
+
+def q4_rounds_weights(dtype, m):
+    """Products of this many f16 rows may round each weight to f16 (tests/decode_reference.py: q4_slack)."""
+    return dtype == F16 and m >= 768
 
 
 @DTYPES
@@ -88,7 +94,7 @@ def test_mat_mul_q4(gpu, case, dtype):
     got = computed(leaf(gpu, x).mat_mul_q4(w.Q4Weights(gpu, codes, scales, z, group)))
     dense = ref.q4_dense(codes, scales, z, group)
     assert got.dtype == dtype
-    ref.close(got, x.astype(np.float64) @ dense, dtype, ref.q4_slack(x, dense, rounded_weights=dtype == F16 and m > 64), str(case))
+    ref.close(got, x.astype(np.float64) @ dense, dtype, ref.q4_slack(x, dense, q4_rounds_weights(dtype, m)), str(case))
 
 
 @DTYPES
@@ -112,14 +118,43 @@ def test_mat_mul_q4_keeps_infinities_and_nan_in_their_rows(gpu):
     w, rng = load_package(), rng_of(12)
     codes, scales, z = ref.q4_weights(rng, 64, 20, 32, False, F16)
     codes[codes == 8] = 9  # no weight is zero: infinity times a weight is infinity
-    for dtype, m in ((F16, 6), (F32, 6), (F16, 70), (F32, 70)):
+    for dtype, m in ((F16, 6), (F32, 6), (F16, 70), (F32, 70), (F16, 800)):
         x = rng.standard_normal((m, 64)).astype(dtype)
         x[1, 3], x[3, 60], x[4, 0], x[4, 1] = np.inf, np.nan, np.inf, -np.inf
         dense = ref.q4_dense(codes, scales, z, 32)
         with np.errstate(invalid="ignore"):
             want = (x.astype(np.float64)[:, :, None] * dense).sum(1)
         finite = np.where(np.isfinite(x), x, 0)
-        ref.close(computed(leaf(gpu, x).mat_mul_q4(w.Q4Weights(gpu, codes, scales, z, 32))), want, dtype, ref.q4_slack(finite, dense, dtype == F16 and m > 64))
+        ref.close(computed(leaf(gpu, x).mat_mul_q4(w.Q4Weights(gpu, codes, scales, z, 32))), want, dtype, ref.q4_slack(finite, dense, q4_rounds_weights(dtype, m)))
+
+
+@DTYPES
+def test_mat_mul_q4_of_rows_that_do_not_start_on_16_bytes(gpu, dtype):
+    """A dense view whose first element is off the alignment that tiles are read with."""
+    w, rng = load_package(), rng_of(14)
+    codes, scales, z = ref.q4_weights(rng, 72, 40, 32, True, F16)
+    weights, dense = w.Q4Weights(gpu, codes, scales, z, 32), ref.q4_dense(codes, scales, z, 32)
+    for rows in (5, 50, 800):
+        x = rng.standard_normal(rows * 72 + 3).astype(dtype)
+        got = computed(leaf(gpu, x).narrow(0, 3, rows * 72).reshape([rows, 72]).mat_mul_q4(weights))
+        ref.close(got, x[3:].reshape(rows, 72).astype(np.float64) @ dense, dtype, ref.q4_slack(x[3:].reshape(rows, 72), dense, q4_rounds_weights(dtype, rows)))
+
+
+def test_mat_mul_q4_with_scales_that_are_not_finite(gpu):
+    """An infinite or NaN scale stays in its column, and in the rows that it belongs to: zeros behind K do not meet it."""
+    w, rng = load_package(), rng_of(15)
+    codes, scales, z = ref.q4_weights(rng, 40, 20, 32, False, F16)
+    codes[codes == 8] = 7
+    scales[1, 3], scales[0, 5], scales[1, 19] = np.inf, np.nan, np.inf
+    for dtype, m in ((F16, 6), (F32, 6), (F16, 40), (F32, 40)):
+        x = np.abs(rng.standard_normal((m, 40))).astype(dtype) + dtype(0.5)
+        codes[32:, 3] = 9  # one sign: the sum is an infinity, not a NaN
+        codes[32:, 19] = 2
+        dense = ref.q4_dense(codes, scales, z, 32)
+        finite = np.where(np.isfinite(dense), dense, 0)
+        with np.errstate(invalid="ignore"):
+            want = (x.astype(np.float64)[:, :, None] * dense).sum(1)
+        ref.close(computed(leaf(gpu, x).mat_mul_q4(w.Q4Weights(gpu, codes, scales, z, 32))), want, dtype, ref.q4_slack(x, finite))
 
 
 def test_mat_mul_q4_without_rows(gpu):
@@ -486,7 +521,7 @@ def test_a_block_serves_a_prompt_and_then_tokens(gpu, dtype):
             continue
         h_qkv, h_q, h_k, h_o, h_y = (t.to_numpy() for t in (qkv, q, k, o, y))
         dense = ref.q4_dense(*into, 32)
-        ref.close(h_qkv, x.astype(np.float64) @ dense, dtype, ref.q4_slack(x, dense, rounded_weights=dtype == F16 and batch * n > 64))
+        ref.close(h_qkv, x.astype(np.float64) @ dense, dtype, ref.q4_slack(x, dense))
         split = h_qkv.reshape(batch, n, heads + 2 * kv, dim).transpose(0, 2, 1, 3)
         for got, part, g in ((h_q, split[:, :heads], gq), (h_k, split[:, heads:heads + kv], gk)):
             ref.close(got, ref.norm_rope(part, g, c, s, 1e-6, lengths), dtype, ref.norm_rope_slack(part, g, 1e-6))
@@ -501,7 +536,7 @@ def test_a_block_serves_a_prompt_and_then_tokens(gpu, dtype):
             ref.close(h_o[b], want, dtype, slack)
         rows = h_o.transpose(0, 2, 1, 3).reshape(batch * n, heads * dim)
         dense = ref.q4_dense(*back, 64)
-        ref.close(h_y, rows.astype(np.float64) @ dense, dtype, ref.q4_slack(rows, dense, rounded_weights=dtype == F16 and batch * n > 64))
+        ref.close(h_y, rows.astype(np.float64) @ dense, dtype, ref.q4_slack(rows, dense))
     if gpu.is_planner:
         pytest.skip("plan-only device: kernels compiled, nothing computed")
     assert cache.lengths() == lengths

@@ -41,6 +41,15 @@ const char* const kQ4Pack =
 const char* const kQ4Dense =
 #include "kernels/q4_dense.hip.inc"
     ;
+const char* const kQ4Numbers =
+#include "kernels/q4_numbers.hip.inc"
+    ;
+const char* const kQ4Rows =
+#include "kernels/q4_rows.hip.inc"
+    ;
+const char* const kQ4Tile =
+#include "kernels/q4_tile.hip.inc"
+    ;
 const char* const kQ4MatMul =
 #include "kernels/q4_mat_mul.hip.inc"
     ;
@@ -100,31 +109,77 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
   const size_t M = x.layout.numel() / w.k, N = w.n, Kp = (w.k + 7) / 8 * 8;
   if (!M) return out;
   if (M > 0xfffffull) throw Error(WKF_ERR_UNSUPPORTED, "mat_mul_q4: more than 2^20 rows");
-  // Many f16 rows: the weights are written out once and the product is mat_mul's.
-  if (x.dtype == DType::F16 && M > 64 && N >= 16 && M * N * Kp >= (size_t(1) << 18)) return mat_mul_q4_dense(w, x, out, M);
-  const bool z = bool(w.zeros);
+  const bool z = bool(w.zeros), h = x.dtype == DType::F16;
+  // Many f16 rows: the weights are written out once, each rounded to f16, and the product is mat_mul's ([1024,4096]x[4096,11008]:
+  // 112 us against 153 in tiles of 4-bit weights, 512 rows 74 against 78, 512 rows of [4096,4096] 42 against 27).
+  if (h && M >= 768 && N >= 16 && M * N * Kp >= (size_t(1) << 18)) return mat_mul_q4_dense(w, x, out, M);
   // the k = 32 steps of a tile that surely share a group, and the group in units of so many
   const size_t step = w.group % 128 == 0 ? 4 : w.group % 64 == 0 ? 2 : 1, units = w.group / (32 * step);
   int shift = -1;
   for (int i = 0; i < 32; i++)
     if (units == size_t(1) << i) shift = i;
-  const size_t mt = M <= 16 ? 1 : M <= 32 ? 2 : 4;
-  std::ostringstream sg;
-  sg << "q4_mat_mul|gfx950|" << dtype_name(x.dtype) << "|s" << dtype_name(w.scale_dtype) << (z ? "|zeros" : "") << "|mt" << mt << "|step" << step << "|shift" << shift;
-  const std::string sig = sg.str();
+  const std::string kind = std::string(dtype_name(x.dtype)) + "|s" + dtype_name(w.scale_dtype) + (z ? "|zeros" : "") + "|step" + std::to_string(step) + (shift < 0 ? "|any" : "");
+  const std::string defines = define("WKF_H", h) + define("WKF_SH", w.scale_dtype == DType::F16) + define("WKF_Z", z) + define("STEP", step) + define("POW2", shift >= 0);
+  std::ostringstream d;
+  d << "m=" << M << " n=" << N << " k=" << w.k << " group=" << w.group;
+  // More than 16 rows share x in the LDS; up to 32 beside few columns do not pay for it (24 rows of [4096,4096]: 9.5 us against 12.4).
+  if (M > (w.tiles_n() <= 256 ? 32 : 16)) {
+    // Tiles of 32 rows x 64 columns with K shared by as many groups of waves as the LDS has room for, until there are more of
+    // them than the chip takes at once; then larger ones, which read x less often ([4096,4096] f16: 128 rows 14.6 us against 26
+    // in tiles of 64 x 128, 256 rows 27.6 against 24; f32 256 rows 48 in 32 x 128 against 68 and 108, 1024 rows 116 in 64 x 256).
+    size_t mt = 2, nt = 1, nw = 4, kw = h ? 4 : 2;
+    constexpr size_t depth = 2;
+    const size_t by32 = (M + 31) / 32;
+    if (h) {
+      if (by32 * ((w.tiles_n() + 3) / 4) > 512) mt = 4, nt = 2, kw = 2;
+    } else if (by32 * ((w.tiles_n() + 3) / 4) > 256) {
+      nt = 2;
+      if (by32 * ((w.tiles_n() + 7) / 8) > 512) mt = 4, nw = 8, kw = 1;
+    }
+    const void* rows = first(x);
+    TensorData planes;
+    if (!h || w.k % 8 || reinterpret_cast<uintptr_t>(rows) % 16) {
+      const size_t pieces = M * (Kp / 8);
+      planes = alloc({size_t(h ? 1 : 3), M, Kp}, DType::F16, false);
+      const std::string rsig = std::string("q4_rows|gfx950|") + dtype_name(x.dtype);
+      wkf_kernel* rk = kernel(rsig, [&] { return std::string(kPrelude) + define("WKF_H", h) + kQ4Rows; });
+      struct {
+        const void* x;
+        void* out;
+        uint32_t m, k, stride, pad;
+      } ra = {rows, ptr(planes.buffer), uint32_t(M), uint32_t(w.k), uint32_t(Kp), 0};
+      launch("q4_rows", rsig, d.str(), rk, grid_dim((pieces + 255) / 256, "mat_mul_q4"), 1, 1, 256, ra);
+      rows = ptr(planes.buffer);
+    }
+    std::ostringstream sg;
+    sg << "q4_tile|gfx950|" << kind << "|" << mt << "x" << nt << "x" << nw << "x" << kw << "|" << depth;
+    const std::string sig = sg.str();
+    wkf_kernel* k = kernel(sig, [&] {
+      return std::string(kPrelude) + defines + define("MT", mt) + define("NT", nt) + define("NW", nw) + define("KW", kw) + define("DEPTH", depth) + kQ4Numbers + kQ4Tile;
+    });
+    struct {
+      const void *x, *codes, *scales, *zeros;
+      void* y;
+      uint32_t m, n, stride, group, groups, tiles_k, shift, tiles_n;
+    } a = {rows, ptr(w.codes), ptr(w.scales), z ? ptr(w.zeros) : nullptr, first(out),
+           uint32_t(M), uint32_t(N), uint32_t(Kp), uint32_t(w.group), uint32_t(w.groups), uint32_t(w.tiles_k()), uint32_t(std::max(shift, 0)), uint32_t(w.tiles_n())};
+    launch("q4_tile", sig, d.str(), k, uint32_t((w.tiles_n() + nw * nt - 1) / (nw * nt)), uint32_t((M + 16 * mt - 1) / (16 * mt)), 1, uint32_t(64 * nw * kw), a);
+    return out;
+  }
+  const size_t mt = M <= 16 ? 1 : 2;
+  // eight waves, two tiles each on their way ([1,4096]x[4096,11008] f16: 9.0 us, 10.7 with four waves, 10.0 with sixteen, 10.8 with four tiles)
+  constexpr size_t waves = 8, pf = 2;
+  const std::string sig = "q4_mat_mul|gfx950|" + kind + "|w" + std::to_string(waves) + "|pf" + std::to_string(pf) + "|mt" + std::to_string(mt);
   wkf_kernel* k = kernel(sig, [&] {
-    return std::string(kPrelude) + define("WKF_H", x.dtype == DType::F16) + define("WKF_SH", w.scale_dtype == DType::F16) + define("WKF_Z", z) + define("MT", mt) +
-           define("STEP", step) + "#define SHIFT " + std::to_string(shift) + "\n" + kQ4MatMul;
+    return std::string(kPrelude) + defines + define("WAVES", waves) + define("PF", pf) + define("MT", mt) + kQ4Numbers + kQ4MatMul;
   });
   struct {
     const void *x, *codes, *scales, *zeros;
     void* y;
-    uint32_t m, n, k, group, groups, tiles_k;
+    uint32_t m, n, k, group, groups, tiles_k, shift, pad;
   } a = {first(x), ptr(w.codes), ptr(w.scales), z ? ptr(w.zeros) : nullptr, first(out),
-         uint32_t(M), uint32_t(N), uint32_t(w.k), uint32_t(w.group), uint32_t(w.groups), uint32_t(w.tiles_k())};
-  std::ostringstream d;
-  d << "m=" << M << " n=" << N << " k=" << w.k << " group=" << w.group;
-  launch("q4_mat_mul", sig, d.str(), k, uint32_t(w.tiles_n()), uint32_t((M + 16 * mt - 1) / (16 * mt)), 1, 512, a);
+         uint32_t(M), uint32_t(N), uint32_t(w.k), uint32_t(w.group), uint32_t(w.groups), uint32_t(w.tiles_k()), uint32_t(std::max(shift, 0)), 0};
+  launch("q4_mat_mul", sig, d.str(), k, uint32_t(w.tiles_n()), uint32_t((M + 16 * mt - 1) / (16 * mt)), 1, uint32_t(64 * waves), a);
   return out;
 }
 
