@@ -642,6 +642,8 @@ class Tensor:
         return self._new(h)
 
     # -- operators of a decoder's attention block (include/wkf_decode.h) ------------
+    _batch = None  # norm_rope: the batch entries of this tensor, once asked for
+
     def mat_mul_q4(self, weights):
         """[..., M, K] times `weights` [K, N] held in 4 bits: wkf_tensor_mat_mul_q4."""
         h = c_void_p()
@@ -652,11 +654,14 @@ class Tensor:
         """The norm of every row of [heads, seq, dim] or [batch, heads, seq, dim] and its rotation, in one pass: row s of
         batch entry b has position positions[b] + s (None: s).  wkf_tensor_norm_rope."""
         if positions is not None:
-            shape = self.shape()
-            if len(positions) != (shape[0] if len(shape) == 4 else 1):
+            if self._batch is None:  # a tensor's shape never changes
+                shape = self.shape()
+                self._batch = shape[0] if len(shape) == 4 else 1
+            if len(positions) != self._batch or min(positions, default=0) < 0:
                 raise WkfError(ERR_INVALID_ARG, "norm_rope: one position per batch entry is required")
+            positions = (c_size_t * len(positions))(*positions)
         h = c_void_p()
-        _check(self._lib.wkf_tensor_norm_rope(self._h, weight._h, cos._h, sin._h, float(eps), None if positions is None else _sizes(positions), byref(h)))
+        _check(self._lib.wkf_tensor_norm_rope(self._h, weight._h, cos._h, sin._h, float(eps), positions, byref(h)))
         return self._new(h)
 
     def attend(self, cache, scale=None, causal=True, counts=None):
@@ -803,9 +808,9 @@ class KvCache:
     def _counts(self, counts):
         if counts is None:
             return None
-        if len(counts) != self.sequences or any(int(n) < 0 for n in counts):
+        if len(counts) != self.sequences or min(counts) < 0:
             raise WkfError(ERR_INVALID_ARG, "one count per sequence is required")
-        return _sizes(counts)
+        return (c_size_t * len(counts))(*counts)
 
     def lengths(self):
         out, n = [], c_size_t()

@@ -4,7 +4,6 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
-#include <sstream>
 
 #include "graph.h"
 
@@ -55,6 +54,12 @@ const char* const kQ4MatMul =
     ;
 
 char* ptr(const BufRef& b) { return static_cast<char*>(wkf_buffer_ptr(b.get())); }
+// "name=value name=value ...": a launch's detail (a stream costs more than the launch's other host work)
+std::string detail(std::initializer_list<std::pair<const char*, size_t>> list) {
+  std::string s;
+  for (const auto& p : list) s.append(s.empty() ? "" : " ").append(p.first).append("=").append(std::to_string(p.second));
+  return s;
+}
 // the first element of a tensor's layout
 char* first(const TensorData& t) { return ptr(t.buffer) + t.layout.offset * dtype_size(t.dtype); }
 
@@ -72,9 +77,7 @@ std::string kv_defines(const KvCache& c, DType dt, size_t nb) {
   return define("WKF_H", dt == DType::F16) + define("D", c.dim) + define("DP", c.dp) + define("T", c.block) + define("NB", nb);
 }
 std::string kv_signature(const char* what, const KvCache& c, DType dt, size_t nb) {
-  std::ostringstream s;
-  s << what << "|gfx950|" << dtype_name(dt) << "|d" << c.dim << "|t" << c.block << "|nb" << nb;
-  return s.str();
+  return std::string(what) + "|gfx950|" + dtype_name(dt) + "|d" + std::to_string(c.dim) + "|t" + std::to_string(c.block) + "|nb" + std::to_string(nb);
 }
 }  // namespace
 
@@ -120,8 +123,7 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
     if (units == size_t(1) << i) shift = i;
   const std::string kind = std::string(dtype_name(x.dtype)) + "|s" + dtype_name(w.scale_dtype) + (z ? "|zeros" : "") + "|step" + std::to_string(step) + (shift < 0 ? "|any" : "");
   const std::string defines = define("WKF_H", h) + define("WKF_SH", w.scale_dtype == DType::F16) + define("WKF_Z", z) + define("STEP", step) + define("POW2", shift >= 0);
-  std::ostringstream d;
-  d << "m=" << M << " n=" << N << " k=" << w.k << " group=" << w.group;
+  const std::string d = detail({{"m", M}, {"n", N}, {"k", w.k}, {"group", w.group}});
   // More than 16 rows share x in the LDS; up to 32 beside few columns do not pay for it (24 rows of [4096,4096]: 9.5 us against 12.4).
   if (M > (w.tiles_n() <= 256 ? 32 : 16)) {
     // Tiles of 32 rows x 64 columns with K shared by as many groups of waves as the LDS has room for, until there are more of
@@ -148,12 +150,10 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
         void* out;
         uint32_t m, k, stride, pad;
       } ra = {rows, ptr(planes.buffer), uint32_t(M), uint32_t(w.k), uint32_t(Kp), 0};
-      launch("q4_rows", rsig, d.str(), rk, grid_dim((pieces + 255) / 256, "mat_mul_q4"), 1, 1, 256, ra);
+      launch("q4_rows", rsig, d, rk, grid_dim((pieces + 255) / 256, "mat_mul_q4"), 1, 1, 256, ra);
       rows = ptr(planes.buffer);
     }
-    std::ostringstream sg;
-    sg << "q4_tile|gfx950|" << kind << "|" << mt << "x" << nt << "x" << nw << "x" << kw << "|" << depth;
-    const std::string sig = sg.str();
+    const std::string sig = "q4_tile|gfx950|" + kind + "|" + std::to_string(mt) + "x" + std::to_string(nt) + "x" + std::to_string(nw) + "x" + std::to_string(kw);
     wkf_kernel* k = kernel(sig, [&] {
       return std::string(kPrelude) + defines + define("MT", mt) + define("NT", nt) + define("NW", nw) + define("KW", kw) + define("DEPTH", depth) + kQ4Numbers + kQ4Tile;
     });
@@ -163,7 +163,7 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
       uint32_t m, n, stride, group, groups, tiles_k, shift, tiles_n;
     } a = {rows, ptr(w.codes), ptr(w.scales), z ? ptr(w.zeros) : nullptr, first(out),
            uint32_t(M), uint32_t(N), uint32_t(Kp), uint32_t(w.group), uint32_t(w.groups), uint32_t(w.tiles_k()), uint32_t(std::max(shift, 0)), uint32_t(w.tiles_n())};
-    launch("q4_tile", sig, d.str(), k, uint32_t((w.tiles_n() + nw * nt - 1) / (nw * nt)), uint32_t((M + 16 * mt - 1) / (16 * mt)), 1, uint32_t(64 * nw * kw), a);
+    launch("q4_tile", sig, d, k, uint32_t((w.tiles_n() + nw * nt - 1) / (nw * nt)), uint32_t((M + 16 * mt - 1) / (16 * mt)), 1, uint32_t(64 * nw * kw), a);
     return out;
   }
   const size_t mt = M <= 16 ? 1 : 2;
@@ -179,7 +179,7 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
     uint32_t m, n, k, group, groups, tiles_k, shift, pad;
   } a = {first(x), ptr(w.codes), ptr(w.scales), z ? ptr(w.zeros) : nullptr, first(out),
          uint32_t(M), uint32_t(N), uint32_t(w.k), uint32_t(w.group), uint32_t(w.groups), uint32_t(w.tiles_k()), uint32_t(std::max(shift, 0)), 0};
-  launch("q4_mat_mul", sig, d.str(), k, uint32_t(w.tiles_n()), uint32_t((M + 16 * mt - 1) / (16 * mt)), 1, uint32_t(64 * waves), a);
+  launch("q4_mat_mul", sig, d, k, uint32_t(w.tiles_n()), uint32_t((M + 16 * mt - 1) / (16 * mt)), 1, uint32_t(64 * waves), a);
   return out;
 }
 
@@ -205,9 +205,7 @@ TensorData Resolver::mat_mul_q4_dense(const Q4& w, const TensorData& x_in, const
     uint32_t n, k, stride, group, groups, tiles_k;
   } a = {ptr(w.codes), ptr(w.scales), z ? ptr(w.zeros) : nullptr, ptr(wt.buffer), uint32_t(N), uint32_t(w.k), uint32_t(Kp), uint32_t(w.group), uint32_t(w.groups), uint32_t(w.tiles_k())};
   if (w.tiles_n() > 65535) throw Error(WKF_ERR_UNSUPPORTED, "mat_mul_q4: more than 2^20 columns");
-  std::ostringstream d;
-  d << "n=" << N << " k=" << w.k << " group=" << w.group;
-  launch("q4_dense", sig, d.str(), k, uint32_t((w.tiles_k() + 3) / 4), uint32_t(w.tiles_n()), 1, 256, a);
+  launch("q4_dense", sig, detail({{"n", N}, {"k", w.k}, {"group", w.group}}), k, uint32_t((w.tiles_k() + 3) / 4), uint32_t(w.tiles_n()), 1, 256, a);
   auto leaf = [&](const TensorData& t) {
     NodeP n = std::make_shared<Node>();
     n->kind = NodeKind::Tensor;
@@ -297,13 +295,15 @@ std::vector<TensorData> Resolver::launch_norm_rope(const std::vector<const Node*
   if (!batch || !seq || !heads) return outs;
   const size_t nb = room_for(std::min(batch, kMaxSequences)), count = members.size();
   const bool full = cos.layout.shape[1] == dim;
-  std::ostringstream sg;
-  sg << "norm_rope|gfx950|" << dtype_name(n0->dtype) << "|w" << dtype_name(ws[0].dtype) << "|t" << dtype_name(cos.dtype) << "|d" << dim << (full ? "|full" : "")
-     << "|nb" << nb << "|x" << count;
-  const std::string sig = sg.str();
+  // the widest pieces of at most 16 bytes that the half is a multiple of, and the lanes that hold a half
+  size_t v = n0->dtype == DType::F16 ? 8 : 4, lanes = 1;
+  while (dim / 2 % v) v /= 2;
+  while (lanes < 64 && lanes * v < dim / 2) lanes *= 2;
+  const std::string sig = std::string("norm_rope|gfx950|") + dtype_name(n0->dtype) + "|w" + dtype_name(ws[0].dtype) + "|t" + dtype_name(cos.dtype) + "|d" + std::to_string(dim) +
+                          (full ? "|full" : "") + "|nb" + std::to_string(nb) + "|x" + std::to_string(count);
   wkf_kernel* k = kernel(sig, [&] {
     return std::string(kPrelude) + define("WKF_H", n0->dtype == DType::F16) + define("WKF_WH", ws[0].dtype == DType::F16) + define("WKF_TH", cos.dtype == DType::F16) +
-           define("D", dim) + define("FULL", full) + define("NB", nb) + define("MEMBERS", count) + kNormRope;
+           define("D", dim) + define("FULL", full) + define("V", v) + define("LANES", lanes) + define("NB", nb) + define("MEMBERS", count) + kNormRope;
   });
   const size_t e = dtype_size(n0->dtype);
   for (size_t b0 = 0; b0 < batch; b0 += kMaxSequences) {
@@ -334,11 +334,10 @@ std::vector<TensorData> Resolver::launch_norm_rope(const std::vector<const Node*
     LaunchRecord r;
     r.kind = "norm_rope";
     r.signature = sig;
-    std::ostringstream d;
-    d << "batch=" << bn << " heads=" << heads << " seq=" << seq << " dim=" << dim << " tensors=" << count;
-    r.detail = d.str();
+    r.detail = detail({{"batch", bn}, {"heads", heads}, {"seq", seq}, {"dim", dim}, {"tensors", count}});
     r.block[0] = 256;
-    r.grid[0] = grid_dim((bn * heads * seq + 3) / 4, "norm_rope");
+    const size_t per = 256 / lanes;
+    r.grid[0] = grid_dim((bn * heads * seq + per - 1) / per, "norm_rope");
     record(std::move(r), k, block);
   }
   return outs;
@@ -424,7 +423,9 @@ void Resolver::append(KvCache& c, const NodeP& kn, const NodeP& vn, const std::v
   if (!total) return;
   const size_t nb = room_for(c.seqs);
   const std::string sig = kv_signature("kv_append", c, kn->dtype, nb);
-  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + kv_defines(c, kn->dtype, nb) + kKvLayout + kKvAppend; });
+  size_t v = kn->dtype == DType::F16 ? 8 : 4;
+  while (c.dim % v) v /= 2;
+  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + define("V", v) + kv_defines(c, kn->dtype, nb) + kKvLayout + kKvAppend; });
   with_room<AppendArgs>(nb, [&](auto& a) {
     for (int i = 0; i < 2; i++) {
       const Strides4 st(in[i].layout);
@@ -515,9 +516,7 @@ TensorData Resolver::run_attend(const NodeP& n) {
       a.tiles = uint32_t(big);
       std::copy(c.len.begin(), c.len.end(), a.len);
       std::copy(args.counts.begin(), args.counts.end(), a.cnt);
-      std::ostringstream d;
-      d << "sequences=" << c.seqs << " heads=" << heads << "/" << c.heads << " rows=" << rows << " dim=" << c.dim << " tiles of 128 rows";
-      launch("attend_prompt", psig, d.str(), pk, grid_dim(big * c.heads * c.seqs, "attend"), 1, 1, 256, a);
+      launch("attend_prompt", psig, detail({{"sequences", c.seqs}, {"heads", heads}, {"kv_heads", c.heads}, {"rows", rows}, {"dim", c.dim}}), pk, grid_dim(big * c.heads * c.seqs, "attend"), 1, 1, 256, a);
     });
     return out;
   }
@@ -548,8 +547,7 @@ TensorData Resolver::run_attend(const NodeP& n) {
   }
   const std::string sig = kv_signature("attend_rows", c, n->dtype, nb) + "|w" + std::to_string(waves);
   wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + define("W", waves) + define("AHEAD", ahead) + kv_defines(c, n->dtype, nb) + kKvLayout + kKvCodes + kAttendRows; });
-  std::ostringstream d;
-  d << "sequences=" << c.seqs << " heads=" << heads << "/" << c.heads << " rows=" << rows << " dim=" << c.dim << " splits=" << splits;
+  const std::string d = detail({{"sequences", c.seqs}, {"heads", heads}, {"kv_heads", c.heads}, {"rows", rows}, {"dim", c.dim}, {"splits", splits}});
   with_room<AttendArgs>(nb, [&](auto& a) {
     const Strides4 st(q.layout);
     a.q = first(q);
@@ -574,7 +572,7 @@ TensorData Resolver::run_attend(const NodeP& n) {
     a.tiles = uint32_t(tiles);
     std::copy(c.len.begin(), c.len.end(), a.len);
     std::copy(args.counts.begin(), args.counts.end(), a.cnt);
-    launch("attend_rows", sig, d.str(), k, grid_dim(splits * tiles, "attend"), uint32_t(c.heads), uint32_t(c.seqs), uint32_t(64 * waves), a);
+    launch("attend_rows", sig, d, k, grid_dim(splits * tiles, "attend"), uint32_t(c.heads), uint32_t(c.seqs), uint32_t(64 * waves), a);
   });
   return out;
 }
