@@ -376,8 +376,8 @@ struct AttendArgs {
   uint64_t sb, sh, ss;
   uint32_t heads, share, rows, seqs, cap, causal;
   float scale;
-  uint32_t splits, span, tiles;
-  uint32_t len[NB], cnt[NB];
+  uint32_t span, tiles, pad;
+  uint32_t len[NB], cnt[NB], start[NB];
 };
 template <size_t NB>
 struct PromptArgs {
@@ -520,26 +520,37 @@ TensorData Resolver::run_attend(const NodeP& n) {
     });
     return out;
   }
-  // How many groups of 32 tokens a workgroup takes.  One workgroup for each compute unit is enough to read at the memory's
-  // rate (16 sequences of 8000 tokens, 32 key heads: 136 us with 256 workgroups, 152 with 1024); where there are fewer
-  // sequences and heads than that, each is split, but joining s parts costs about as much as reading s groups, so no
-  // finer than its square root (one sequence, 8 key heads: 4000 tokens 16.6 us in 32 parts, 11.7 in 11; 16000 tokens 21.4 us
-  // in 32 parts, 19.3 in 16).  Up to 16 groups stay whole: the join alone takes 3 us.
+  // How many groups of 32 tokens a workgroup takes: so few that there are nearly as many workgroups as the chip holds at once
+  // (512; large heads leave registers for 256), and no more, where a second round would begin (16 sequences of 17000 to 32768
+  // tokens, 8 key heads: 149 us, against 174 with 304 workgroups; 8 sequences of up to 3000, 8 heads of 256: 26 us, 33 with 512).  Joining s parts costs about as much as reading s groups, so a few long sequences
+  // are split no finer than the square root of twice their groups (one sequence, 8 key heads: 4000 tokens 16.6 us in 32 parts,
+  // 11.9 in 8; 16000 tokens 21.4 us in 32 parts, 19.3 in 16).  Up to 16 groups stay whole: the join alone takes 3 us.
   size_t total = 0, longest = 0;
   for (uint32_t n : c.len) {
     total += (n + 31) / 32;
     longest = std::max<size_t>(longest, (n + 31) / 32);
   }
-  constexpr size_t waves = 4, ahead = 2, target = 256;
-  size_t span = (total * c.heads * tiles + target - 1) / target;
-  span = std::max(span, longest <= 16 ? longest : size_t(std::ceil(std::sqrt(double(longest)))));
+  constexpr size_t waves = 4, ahead = 2;
+  const size_t each = c.heads * tiles, resident = c.dp <= 128 ? 512 : 256;
+  size_t span = longest <= 16 ? longest : std::max((total * each + resident - 1) / resident, size_t(std::ceil(std::sqrt(2.0 * double(longest)))));
   span = std::max(waves, (span + waves - 1) / waves * waves);
-  const size_t splits = std::max<size_t>(1, (longest + span - 1) / span);
+  for (;; span += waves) {
+    size_t workgroups = 0;
+    for (uint32_t n : c.len) workgroups += each * (((n + 31) / 32 + span - 1) / span);
+    if (workgroups <= resident || span >= longest) break;
+  }
+  std::vector<uint32_t> start;  // the splits of the sequences before each
+  size_t splits = 0;
+  for (uint32_t n : c.len) {
+    start.push_back(uint32_t(splits));
+    splits += std::max<size_t>(1, ((n + 31) / 32 + span - 1) / span);
+  }
+  const bool split = splits > c.seqs;
   TensorData part, stat;
-  if (splits > 1) {
-    part = alloc({splits, c.seqs, c.heads, tiles, 16, c.dp}, DType::F32, false);
-    stat = alloc({splits, c.seqs, c.heads, tiles, 32}, DType::F32, false);
-    const size_t counters = c.seqs * c.heads * tiles;
+  if (split) {
+    part = alloc({splits, each, 16, c.dp}, DType::F32, false);
+    stat = alloc({splits, each, 32}, DType::F32, false);
+    const size_t counters = c.seqs * each;
     if (counters > c.counters) {  // zeros, and every launch leaves zeros
       c.done = alloc({counters}, DType::F32, true).buffer;
       c.counters = counters;
@@ -554,9 +565,9 @@ TensorData Resolver::run_attend(const NodeP& n) {
     a.out = first(out);
     a.codes = ptr(c.codes);
     a.scales = ptr(c.scales);
-    a.part = splits > 1 ? ptr(part.buffer) : nullptr;
-    a.stat = splits > 1 ? ptr(stat.buffer) : nullptr;
-    a.done = splits > 1 ? ptr(c.done) : nullptr;
+    a.part = split ? ptr(part.buffer) : nullptr;
+    a.stat = split ? ptr(stat.buffer) : nullptr;
+    a.done = split ? ptr(c.done) : nullptr;
     a.sb = st.b;
     a.sh = st.h;
     a.ss = st.s;
@@ -567,12 +578,12 @@ TensorData Resolver::run_attend(const NodeP& n) {
     a.cap = uint32_t(c.cap);
     a.causal = args.causal;
     a.scale = args.scale;
-    a.splits = uint32_t(splits);
     a.span = uint32_t(span);
     a.tiles = uint32_t(tiles);
     std::copy(c.len.begin(), c.len.end(), a.len);
     std::copy(args.counts.begin(), args.counts.end(), a.cnt);
-    launch("attend_rows", sig, d, k, grid_dim(splits * tiles, "attend"), uint32_t(c.heads), uint32_t(c.seqs), uint32_t(64 * waves), a);
+    std::copy(start.begin(), start.end(), a.start);
+    launch("attend_rows", sig, d, k, grid_dim(splits * each, "attend"), 1, 1, uint32_t(64 * waves), a);
   });
   return out;
 }
