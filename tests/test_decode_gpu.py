@@ -219,6 +219,24 @@ def test_norm_rope_of_columns_zeros_and_infinities(gpu):
     want = ref.norm_rope(x.transpose(0, 2, 1), weight, c, s, 1e-5, [0])
     rows = np.ones((2, 6), bool)
     rows[1, 3] = False  # 1e30 squared leaves f32: the norm is infinite and the row zero
+def test_norm_rope_of_a_norm_rope_beside_it(gpu):
+    """A root that is computed from another one with the same tables is a launch of its own, after it."""
+    w, rng = load_package(), rng_of(23)
+    x = rng.standard_normal((2, 7, 64)).astype(F32)
+    c, s = (rng.standard_normal((7, 32)).astype(F32) for _ in range(2))
+    g = np.ones(64, F32)
+    tg, tc, ts = (leaf(gpu, v) for v in (g, c, s))
+    once = leaf(gpu, x).norm_rope(tg, tc, ts, 1e-5)
+    twice = once.norm_rope(tg, tc, ts, 1e-5)
+    outs = [w.Tensor.zeros(gpu, x.shape) for _ in range(2)]
+    w.materialize_into([twice, once], outs)
+    assert [k.kind for k in twice.kernels()] == ["norm_rope"] * 2
+    got = computed(*outs)
+    first = ref.norm_rope(x, g, c, s, 1e-5, [0])
+    ref.close(got[1], first, F32, ref.norm_rope_slack(x, g, 1e-5))
+    ref.close(got[0], ref.norm_rope(got[1], g, c, s, 1e-5, [0]), F32, ref.norm_rope_slack(got[1], g, 1e-5))
+
+
     assert np.all(got[1, 3] == 0) and np.all(got[0, 1] == 0) and np.all(np.isnan(got[1, 2]))
     ref.close(got[rows], want[rows], F32, ref.norm_rope_slack(x.transpose(0, 2, 1), weight, 1e-5)[rows])
 

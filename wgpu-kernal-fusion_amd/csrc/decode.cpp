@@ -248,6 +248,21 @@ size_t nr_dim(const Node* n, size_t i) {
 }  // namespace
 
 void Resolver::join_norm_ropes(const std::vector<NodeP>& roots) {
+namespace {
+// whether the value of `n` is computed from that of `from`
+bool depends(const NodeP& n, const Node* from, std::set<const Node*>* seen) {
+  if (!n || !seen->insert(n.get()).second) return false;
+  if (n.get() == from) return true;
+  for (const NodeP& m : n->more)
+    if (depends(m, from, seen)) return true;
+  return depends(n->a, from, seen) || depends(n->b, from, seen);
+}
+bool depends(const Node* n, const Node* from) {
+  std::set<const Node*> seen;
+  return depends(n->a, from, &seen) || depends(n->more[0], from, &seen) || depends(n->more[1], from, &seen) || depends(n->more[2], from, &seen);
+}
+}  // namespace
+
   std::vector<std::vector<const Node*>> groups;
   std::set<const Node*> seen;
   for (const NodeP& r : roots) {
@@ -258,7 +273,8 @@ void Resolver::join_norm_ropes(const std::vector<NodeP>& roots) {
       const NormRopeArgs &x = norm_rope_args(o), &y = norm_rope_args(n);
       if (g.size() < kMaxMembers && o->dtype == n->dtype && nr_dim(o, 0) == nr_dim(n, 0) && nr_dim(o, 2) == nr_dim(n, 2) && nr_dim(o, 3) == nr_dim(n, 3) &&
           o->more[0]->dtype == n->more[0]->dtype && o->more[1] == n->more[1] && o->more[2] == n->more[2] &&
-          memcmp(&x.eps, &y.eps, sizeof(float)) == 0 && x.positions == y.positions) {
+          memcmp(&x.eps, &y.eps, sizeof(float)) == 0 && x.positions == y.positions &&
+          std::none_of(g.begin(), g.end(), [&](const Node* m) { return depends(n, m) || depends(m, n); })) {
         g.push_back(n);
         placed = true;
         break;
