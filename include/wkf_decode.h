@@ -51,7 +51,8 @@ int wkf_q4_new(wkf_device* dev, size_t k, size_t n, size_t group, const void* co
 /* Tensors recorded with the weights keep them alive. */
 void wkf_q4_free(wkf_q4* w);
 int wkf_q4_shape(const wkf_q4* w, size_t* k, size_t* n, size_t* group);
-/* x [..., M, k] times W [k, n]: [..., M, n] in x's dtype. */
+/* x [..., M, k] times W [k, n]: [..., M, n] in x's dtype, with at most 2^20 - 1 rows of x in all.  With many rows of f16 each
+ * weight may be rounded to f16 first, if none of them is too large or too small for its normal numbers. */
 int wkf_tensor_mat_mul_q4(const wkf_tensor* x, const wkf_q4* w, wkf_tensor** out);
 
 /* ---- the norm of a head and its rotation ---- */

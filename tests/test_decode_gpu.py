@@ -157,6 +157,17 @@ def test_mat_mul_q4_with_scales_that_are_not_finite(gpu):
         ref.close(computed(leaf(gpu, x).mat_mul_q4(w.Q4Weights(gpu, codes, scales, z, 32))), want, dtype, ref.q4_slack(x, finite))
 
 
+@pytest.mark.parametrize("scale", [2e4, 1e-7, 3e-5], ids=str)
+def test_mat_mul_q4_of_weights_beyond_f16(gpu, scale):
+    """Weights that f16 could not hold, or not with all its bits, meet many rows of f16."""
+    w, rng = load_package(), rng_of(16)
+    codes, scales, z = ref.q4_weights(rng, 96, 40, 32, True, F32)
+    scales = (scales * F32(scale / 0.02)).astype(F32)
+    x = (rng.standard_normal((800, 96)) * min(1.0, 1e-3 / scale)).astype(F16)
+    dense = ref.q4_dense(codes, scales, z, 32)
+    ref.close(computed(leaf(gpu, x).mat_mul_q4(w.Q4Weights(gpu, codes, scales, z, 32))), x.astype(np.float64) @ dense, F16, ref.q4_slack(x, dense))
+
+
 def test_mat_mul_q4_without_rows(gpu):
     w = load_package()
     codes, scales, z = ref.q4_weights(rng_of(13), 64, 20, 32, False, F16)

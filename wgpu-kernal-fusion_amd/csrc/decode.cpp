@@ -114,8 +114,9 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
   if (M > 0xfffffull) throw Error(WKF_ERR_UNSUPPORTED, "mat_mul_q4: more than 2^20 rows");
   const bool z = bool(w.zeros), h = x.dtype == DType::F16;
   // Many f16 rows: the weights are written out once, each rounded to f16, and the product is mat_mul's ([1024,4096]x[4096,11008]:
-  // 112 us against 153 in tiles of 4-bit weights, 512 rows 74 against 78, 512 rows of [4096,4096] 42 against 27).
-  if (h && M >= 768 && N >= 16 && M * N * Kp >= (size_t(1) << 18)) return mat_mul_q4_dense(w, x, out, M);
+  // 112 us against 153 in tiles of 4-bit weights, 512 rows 74 against 78, 512 rows of [4096,4096] 42 against 27).  Weights that
+  // would overflow or lose bits there stay in the tiles, which round none.
+  if (h && w.fits_f16 && M >= 768 && N >= 16 && w.tiles_n() <= 65535 && M * N * Kp >= (size_t(1) << 18)) return mat_mul_q4_dense(w, x, out, M);
   // the k = 32 steps of a tile that surely share a group, and the group in units of so many
   const size_t step = w.group % 128 == 0 ? 4 : w.group % 64 == 0 ? 2 : 1, units = w.group / (32 * step);
   int shift = -1;
@@ -204,7 +205,6 @@ TensorData Resolver::mat_mul_q4_dense(const Q4& w, const TensorData& x_in, const
     void* out;
     uint32_t n, k, stride, group, groups, tiles_k;
   } a = {ptr(w.codes), ptr(w.scales), z ? ptr(w.zeros) : nullptr, ptr(wt.buffer), uint32_t(N), uint32_t(w.k), uint32_t(Kp), uint32_t(w.group), uint32_t(w.groups), uint32_t(w.tiles_k())};
-  if (w.tiles_n() > 65535) throw Error(WKF_ERR_UNSUPPORTED, "mat_mul_q4: more than 2^20 columns");
   launch("q4_dense", sig, detail({{"n", N}, {"k", w.k}, {"group", w.group}}), k, uint32_t((w.tiles_k() + 3) / 4), uint32_t(w.tiles_n()), 1, 256, a);
   auto leaf = [&](const TensorData& t) {
     NodeP n = std::make_shared<Node>();

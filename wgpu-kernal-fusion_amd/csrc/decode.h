@@ -25,6 +25,7 @@ struct Q4 {
   size_t k = 0, n = 0, group = 0, groups = 0;
   DType scale_dtype = DType::F16;
   BufRef codes, scales, zeros;  // zeros: none = 8 everywhere
+  bool fits_f16 = false;        // every weight is zero, or within the normal numbers of f16 when it is rounded to that
   size_t tiles_k() const { return (k + 127) / 128; }
   size_t tiles_n() const { return (n + 15) / 16; }
 };

@@ -163,6 +163,12 @@ int wkf_q4_new(wkf_device* dev, size_t k, size_t n, size_t group, const void* co
     if (zeros && high(zeros, gn)) invalid("wkf_q4_new: a zero point is larger than 15");
     const size_t tiles = times(w->tiles_k(), w->tiles_n(), who), padded = times(w->tiles_n() * 16, w->groups, who);
     if (tiles > 0x7fffffffull) invalid("wkf_q4_new: too large");
+    // a weight is a scale times a whole number of 0 .. 15 (a NaN fails both comparisons)
+    w->fits_f16 = true;
+    for (size_t i = 0; i < gn; i++) {
+      const float s = w->scale_dtype == DType::F16 ? float(static_cast<const _Float16*>(scales)[i]) : static_cast<const float*>(scales)[i];
+      w->fits_f16 &= s == 0.f || (std::fabs(s) >= 0x1p-14f && std::fabs(s) <= 65504.f / 15);
+    }
     w->codes = buffer(dev, times(tiles, 1024, who));
     w->scales = buffer(dev, padded * es);
     if (zeros) w->zeros = buffer(dev, padded);
