@@ -491,6 +491,63 @@ def test_attend_over_zero_blocks_and_what_lies_behind_the_end(gpu, rows, kv, dty
     assert np.all(got[0, 2:4] == 0)
 
 
+@pytest.mark.parametrize("scale", [0.0, 0.125])
+def test_attend_with_many_rows_before_a_block_of_zero_keys_and_large_values(gpu, scale):
+    """Rows that end before a block are not touched by its scales, also where those scales make every score 0."""
+    w, rng = load_package(), rng_of(45)
+    cache = w.KvCache(gpu, 4, 16, 64, 64, 32)
+    k, v = (rng.standard_normal((4, 16, 64, 64)).astype(F32) for _ in range(2))
+    k[:, :, 32:] = 0
+    v[:, :, 32:] *= F32(1e9)  # f16 holds no result of the rows that see them
+    cache.append(leaf(gpu, k), leaf(gpu, v))
+    q = rng.standard_normal((4, 128, 64, 64)).astype(F16)
+    out = leaf(gpu, q).attend(cache, scale)
+    got, held = computed(out, cache.values(0, 32, w.F32))
+    assert [i.kind for i in out.kernels()] == ["attend_prompt"]
+    for b in range(4):
+        case = (q[b, :, :32], held[0, b].astype(np.float64), held[1, b].astype(np.float64), scale, True, 32, 32)
+        want, slack = ref.attend(*case)
+        ref.close(got[b, :, :32], want, F16, slack + ref.f16_weights_slack(*case), f"sequence {b}")
+
+
+@DTYPES
+def test_attend_in_a_cache_of_more_than_32_bits_of_bytes(gpu, dtype):
+    """The last head's keys and all values lie behind 4 GiB; one sequence of a few is long, the others short."""
+    check_attend(gpu, dtype, [3000, 1, 64], 3, 3, 128, 64, 1, capacity=5 << 20)
+    check_attend(gpu, dtype, [200, 130, 70], 3, 3, 128, 64, 70, capacity=5 << 20)
+
+
+def test_attend_over_many_short_sequences_and_a_long_one(gpu):
+    check_attend(gpu, F16, [4000] + [3, 40, 0, 17] * 30, 8, 8, 64, 32, 1)
+
+
+def test_the_operators_under_the_reference_s_own_fusion(gpu):
+    """Nothing is shared or joined there; the values are the same."""
+    w, rng = load_package(), rng_of(46)
+    codes, scales, z = ref.q4_weights(rng, 128, 256, 32, True, F16)
+    weights = w.Q4Weights(gpu, codes, scales, z, 32)
+    x = leaf(gpu, rng.standard_normal((800, 128)).astype(F16))
+    c, s = (leaf(gpu, rng.standard_normal((800, 32)).astype(F32)) for _ in range(2))
+    g = leaf(gpu, np.ones(64, F32))
+    got = []
+    for mode in (w.FUSION_TREE, w.FUSION_REFERENCE):
+        gpu.set_fusion(mode)
+        try:
+            cache = w.KvCache(gpu, 1, 2, 64, 800, 32)
+            y = x.mat_mul_q4(weights)
+            q, k = (y.narrow(1, at, n * 64).reshape([800, n, 64]).transpose(0, 1).norm_rope(g, c, s, 1e-5) for at, n in ((0, 2), (128, 2)))
+            cache.append(k, y.narrow(1, 128, 128).reshape([800, 2, 64]).transpose(0, 1))
+            lazy = [q, k, q.attend(cache, 0.125), cache.values(0, 800, w.F16)]
+            outs = [w.Tensor.zeros(gpu, t.shape(), w.F16) for t in lazy]
+            w.materialize_into(lazy, outs)
+            got += outs
+        finally:
+            gpu.set_fusion(w.FUSION_TREE)
+    values = computed(*got)
+    for i in range(4):
+        assert np.array_equal(values[i], values[4 + i])
+
+
 def test_attend_of_an_empty_cache_and_of_no_rows(gpu):
     w = load_package()
     cache = w.KvCache(gpu, 2, 2, 64, 64, 32)
