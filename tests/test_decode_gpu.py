@@ -219,17 +219,6 @@ def test_norm_rope_of_a_projection_in_one_launch(gpu, dtype):
         assert np.array_equal(got[i], got[2 + i])  # alone: the same values
 
 
-def test_norm_rope_of_columns_zeros_and_infinities(gpu):
-    rng = rng_of(22)
-    x = rng.standard_normal((2, 64, 6)).astype(F32)  # the last dimension of the view is not dense
-    x[0, :, 1] = 0
-    x[1, 5, 2], x[1, 7, 3] = np.nan, 1e30
-    c, s = (rng.standard_normal((6, 32)).astype(F32) for _ in range(2))
-    weight = np.ones(64, F32)
-    got = computed(leaf(gpu, x).transpose(1, 2).norm_rope(leaf(gpu, weight), leaf(gpu, c), leaf(gpu, s), 1e-5))
-    want = ref.norm_rope(x.transpose(0, 2, 1), weight, c, s, 1e-5, [0])
-    rows = np.ones((2, 6), bool)
-    rows[1, 3] = False  # 1e30 squared leaves f32: the norm is infinite and the row zero
 def test_norm_rope_of_a_norm_rope_beside_it(gpu):
     """A root that is computed from another one with the same tables is a launch of its own, after it."""
     w, rng = load_package(), rng_of(23)
@@ -248,6 +237,17 @@ def test_norm_rope_of_a_norm_rope_beside_it(gpu):
     ref.close(got[0], ref.norm_rope(got[1], g, c, s, 1e-5, [0]), F32, ref.norm_rope_slack(got[1], g, 1e-5))
 
 
+def test_norm_rope_of_columns_zeros_and_infinities(gpu):
+    rng = rng_of(22)
+    x = rng.standard_normal((2, 64, 6)).astype(F32)  # the last dimension of the view is not dense
+    x[0, :, 1] = 0
+    x[1, 5, 2], x[1, 7, 3] = np.nan, 1e30
+    c, s = (rng.standard_normal((6, 32)).astype(F32) for _ in range(2))
+    weight = np.ones(64, F32)
+    got = computed(leaf(gpu, x).transpose(1, 2).norm_rope(leaf(gpu, weight), leaf(gpu, c), leaf(gpu, s), 1e-5))
+    want = ref.norm_rope(x.transpose(0, 2, 1), weight, c, s, 1e-5, [0])
+    rows = np.ones((2, 6), bool)
+    rows[1, 3] = False  # 1e30 squared leaves f32: the norm is infinite and the row zero
     assert np.all(got[1, 3] == 0) and np.all(got[0, 1] == 0) and np.all(np.isnan(got[1, 2]))
     ref.close(got[rows], want[rows], F32, ref.norm_rope_slack(x.transpose(0, 2, 1), weight, 1e-5)[rows])
 

@@ -165,6 +165,12 @@ def test_refusals_of_the_cache_and_its_attention(wkf, planner):
             cache.values(*args)
     with refused(wkf, "dtype"):
         cache.values(0, 1, 5)
+    with refused(wkf, "too many rows"):
+        zeros(wkf, planner, (2, 8, 64)).broadcast((2, 8, (1 << 30) - 1, 64)).attend(cache, counts=[1, 1])
+    with pytest.raises(TypeError):
+        zeros(wkf, planner, (2, 4, 1, 64)).attend(cache, counts=[1.5, 1])
+    for counts in ([np.int64(1), np.int32(1)], (1, 0)):  # whole numbers of any kind
+        assert zeros(wkf, planner, (2, 4, 1, 64)).attend(cache, counts=counts).shape() == (2, 4, 1, 64)
     with refused(wkf, "no such sequence"):
         cache.reset(2)
     assert lib.wkf_kv_cache_reset(cache._h, 2) == wkf.ERR_INVALID_ARG and lib.wkf_kv_cache_length(cache._h, 2, ctypes.byref(ctypes.c_size_t())) == wkf.ERR_INVALID_ARG

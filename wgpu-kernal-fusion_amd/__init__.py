@@ -13,6 +13,7 @@ compiles kernels but cannot run them (host-side tests only).
 from __future__ import annotations
 
 import ctypes
+import operator
 import os
 from ctypes import POINTER, byref, c_char_p, c_float, c_int, c_size_t, c_uint64, c_void_p
 
@@ -659,7 +660,7 @@ class Tensor:
                 self._batch = shape[0] if len(shape) == 4 else 1
             if len(positions) != self._batch or min(positions, default=0) < 0:
                 raise WkfError(ERR_INVALID_ARG, "norm_rope: one position per batch entry is required")
-            positions = (c_size_t * len(positions))(*positions)
+            positions = (c_size_t * len(positions))(*map(operator.index, positions))
         h = c_void_p()
         _check(self._lib.wkf_tensor_norm_rope(self._h, weight._h, cos._h, sin._h, float(eps), positions, byref(h)))
         return self._new(h)
@@ -810,7 +811,7 @@ class KvCache:
             return None
         if len(counts) != self.sequences or min(counts) < 0:
             raise WkfError(ERR_INVALID_ARG, "one count per sequence is required")
-        return (c_size_t * len(counts))(*counts)
+        return (c_size_t * len(counts))(*map(operator.index, counts))
 
     def lengths(self):
         out, n = [], c_size_t()

@@ -68,8 +68,9 @@ std::string define(const char* name, size_t v) { return std::string("#define ") 
 // Lengths of up to 8, 64 or 256 sequences travel in an argument block: three kernels, so that the usual few do not carry 2 KB.
 size_t room_for(size_t sequences) { return sequences <= 8 ? 8 : sequences <= 64 ? 64 : kMaxSequences; }
 
-uint32_t grid_dim(size_t v, const char* what) {
-  if (v > 0x7fffffffull) throw Error(WKF_ERR_UNSUPPORTED, std::string(what) + ": too many workgroups");
+// workgroups of `threads` along x: a launch has less than 2^32 threads there
+uint32_t grid_dim(size_t v, const char* what, size_t threads = 256) {
+  if (v > 0xffffffffull / threads) throw Error(WKF_ERR_UNSUPPORTED, std::string(what) + ": too many workgroups");
   return uint32_t(v);
 }
 
@@ -101,7 +102,7 @@ void Resolver::pack_q4(Q4& w, const TensorData& codes, const TensorData& scales,
     uint32_t k, n, groups, tiles_k;
   } a = {ptr(codes.buffer), ptr(scales.buffer), z ? ptr(zeros.buffer) : nullptr, ptr(w.codes), ptr(w.scales), z ? ptr(w.zeros) : nullptr,
          uint32_t(w.k), uint32_t(w.n), uint32_t(w.groups), uint32_t(w.tiles_k())};
-  launch("q4_pack", sig, "", k, grid_dim(w.tiles_k() * w.tiles_n(), "q4"), 1, 1, 64, a);
+  launch("q4_pack", sig, "", k, grid_dim(w.tiles_k() * w.tiles_n(), "q4", 64), 1, 1, 64, a);
 }
 
 TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
@@ -247,7 +248,6 @@ size_t nr_dim(const Node* n, size_t i) {
 }
 }  // namespace
 
-void Resolver::join_norm_ropes(const std::vector<NodeP>& roots) {
 namespace {
 // whether the value of `n` is computed from that of `from`
 bool depends(const NodeP& n, const Node* from, std::set<const Node*>* seen) {
@@ -263,6 +263,7 @@ bool depends(const Node* n, const Node* from) {
 }
 }  // namespace
 
+void Resolver::join_norm_ropes(const std::vector<NodeP>& roots) {
   std::vector<std::vector<const Node*>> groups;
   std::set<const Node*> seen;
   for (const NodeP& r : roots) {
@@ -550,10 +551,16 @@ TensorData Resolver::run_attend(const NodeP& n) {
   const size_t each = c.heads * tiles, resident = c.dp <= 128 ? 512 : 256;
   size_t span = longest <= 16 ? longest : std::max((total * each + resident - 1) / resident, size_t(std::ceil(std::sqrt(2.0 * double(longest)))));
   span = std::max(waves, (span + waves - 1) / waves * waves);
-  for (;; span += waves) {
+  // Sequences and heads that are more than that by themselves stay whole (64 of 2000 to 4000 tokens, 8 heads: 81 us, 88 in
+  // parts), unless some are much longer than the average: half as many again are for those (one of 32000 tokens among 63 of
+  // 300: 32 us against 194).  Many times as many keep the chip busy in any case, and their parts would take too much memory.
+  const size_t units = c.seqs * each, most = std::max(resident, units + (longest > 2 * total / c.seqs ? resident / 2 : 0));
+  if (units > 32 * resident) span = std::max(span, (longest + waves - 1) / waves * waves);
+  while (span < longest) {
     size_t workgroups = 0;
-    for (uint32_t n : c.len) workgroups += each * (((n + 31) / 32 + span - 1) / span);
-    if (workgroups <= resident || span >= longest) break;
+    for (uint32_t n : c.len) workgroups += each * std::max<size_t>(1, ((n + 31) / 32 + span - 1) / span);
+    if (workgroups <= most) break;
+    span += (span / 16 + waves) / waves * waves;
   }
   std::vector<uint32_t> start;  // the splits of the sequences before each
   size_t splits = 0;
@@ -566,10 +573,9 @@ TensorData Resolver::run_attend(const NodeP& n) {
   if (split) {
     part = alloc({splits, each, 16, c.dp}, DType::F32, false);
     stat = alloc({splits, each, 32}, DType::F32, false);
-    const size_t counters = c.seqs * each;
-    if (counters > c.counters) {  // zeros, and every launch leaves zeros
-      c.done = alloc({counters}, DType::F32, true).buffer;
-      c.counters = counters;
+    if (units > c.counters) {  // zeros, and every launch leaves zeros
+      c.done = alloc({units}, DType::F32, true).buffer;
+      c.counters = units;
     }
   }
   const std::string sig = kv_signature("attend_rows", c, n->dtype, nb) + "|w" + std::to_string(waves);

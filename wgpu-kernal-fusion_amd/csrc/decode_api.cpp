@@ -355,6 +355,7 @@ int wkf_tensor_attend(const wkf_tensor* q, wkf_kv_cache* c, float scale, int cau
     cache_shape(*c->c, q, who, "q", &heads, &rows);
     if (!heads || heads % c->c->heads) invalid("attend: the query heads must be a multiple of the cache's");
     if (heads > 65535) invalid("attend: at most 65535 query heads");
+    if (heads / c->c->heads * rows > 0x7fffff00ull) invalid("attend: too many rows for a key head");
     if (!(scale >= 0.f) || std::isinf(scale)) invalid("attend: the scale must be finite and not negative");
     const std::vector<size_t> n = counts_of(*c->c, counts, rows, who);
     NodeP t = make(NodeKind::Attend, q->node->dtype, q->node->shape);
