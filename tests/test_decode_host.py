@@ -3,6 +3,8 @@ kernel, and the lengths a cache keeps on the host.  On a plan-only device kernel
 import ctypes
 import os
 import re
+import shutil
+import subprocess
 
 import numpy as np
 import pytest
@@ -163,14 +165,14 @@ def test_refusals_of_the_cache_and_its_attention(wkf, planner):
     for args in ((0, 41), (40, 1), (41, 0)):
         with refused(wkf, "capacity"):
             cache.values(*args)
-    with refused(wkf, "dtype"):
-        cache.values(0, 1, 5)
     with refused(wkf, "too many rows"):
         zeros(wkf, planner, (2, 8, 64)).broadcast((2, 8, (1 << 30) - 1, 64)).attend(cache, counts=[1, 1])
     with pytest.raises(TypeError):
         zeros(wkf, planner, (2, 4, 1, 64)).attend(cache, counts=[1.5, 1])
     for counts in ([np.int64(1), np.int32(1)], (1, 0)):  # whole numbers of any kind
         assert zeros(wkf, planner, (2, 4, 1, 64)).attend(cache, counts=counts).shape() == (2, 4, 1, 64)
+    with refused(wkf, "dtype"):
+        cache.values(0, 1, 5)
     with refused(wkf, "no such sequence"):
         cache.reset(2)
     assert lib.wkf_kv_cache_reset(cache._h, 2) == wkf.ERR_INVALID_ARG and lib.wkf_kv_cache_length(cache._h, 2, ctypes.byref(ctypes.c_size_t())) == wkf.ERR_INVALID_ARG
@@ -250,3 +252,49 @@ def test_extern_block_of_the_guide_matches_the_header():
     block = block[:block.index("```")]
     rust = {m.group(1): len([p for p in m.group(2).split(",") if p.strip()]) for m in re.finditer(r"pub fn (wkf_\w+)\s*\(([^)]*)\)", block)}
     assert rust == c
+
+
+FACADE = r"""
+    #include <cstdio>
+    #include <wkf_decode.hpp>
+    using namespace wkf;
+    template <class F>
+    static int refused(F f) {
+      try { f(); } catch (const Error& e) { return e.code; }
+      return 0;
+    }
+    int main() {
+      auto dev = Device::planner();
+      std::vector<Half> scales(2 * 128, Half::from_float(0.5f));
+      auto w = Q4Weights::make<F16>(dev, 64, 128, 32, std::vector<uint8_t>(64 * 128, 3), scales);
+      auto y = mat_mul_q4(zeros<2, F16>(dev, {3, 64}), w);
+      KvCache cache(dev, 1, 2, 64, 100, 32);
+      Tensor<1, F32> g(dev, {64}, std::vector<float>(64, 1.0f));
+      auto table = zeros<2, F32>(dev, {9, 32});
+      auto k = norm_rope(zeros<3, F16>(dev, {2, 3, 64}), g, table, table, 1e-5f, {6});
+      cache.append(k, k);
+      cache.append(k, k, {2});
+      auto q = norm_rope(zeros<4, F16>(dev, {1, 4, 3, 64}), g, table, table, 1e-5f);
+      auto o = attend(q, cache, 0.125f);
+      auto out = zeros<4, F16>(dev, {1, 4, 3, 64});
+      materialize_into(o, out);
+      const bool fine = y.shape() == std::array<size_t, 2>{3, 128} && cache.lengths() == std::vector<size_t>{5} && cache.values<F32>(0, 5).shape()[3] == 5 &&
+          refused([&] { cache.append(k, k, {1, 1}); }) == WKF_ERR_INVALID_ARG && refused([&] { norm_rope(k, g, table, table, 1e-5f, {7}); }) == WKF_ERR_INVALID_ARG &&
+          refused([&] { Q4Weights::make<F16>(dev, 64, 128, 32, {}, scales); }) == WKF_ERR_INVALID_ARG && refused([&] { attend(q, cache, 0.125f, true, {4}); }) == WKF_ERR_INVALID_ARG;
+      cache.reset();
+      std::printf("%s\n", fine && cache.lengths()[0] == 0 ? "OK" : "FAILED");
+      return 0;
+    }
+"""
+
+
+def test_the_typed_facade_compiles_and_plans(tmp_path):
+    gxx, libdir = shutil.which("g++"), os.path.join(ROOT, "wgpu-kernal-fusion_amd")
+    if gxx is None:
+        pytest.skip("no g++ on this machine")
+    (tmp_path / "facade.cpp").write_text(FACADE)
+    r = subprocess.run([gxx, "-std=c++17", "-O1", "-Wall", "-Wextra", "-Werror", "-I", os.path.join(ROOT, "include"), str(tmp_path / "facade.cpp"), "-o", str(tmp_path / "facade"),
+                        "-L", libdir, "-lwkf_hip", f"-Wl,-rpath,{libdir}"], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout + r.stderr
+    r = subprocess.run([str(tmp_path / "facade")], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and r.stdout.strip() == "OK", r.stdout + r.stderr
