@@ -13,8 +13,8 @@ compiles kernels but cannot run them (host-side tests only).
 from __future__ import annotations
 
 import ctypes
-import operator
 import os
+from array import array
 from ctypes import POINTER, byref, c_char_p, c_float, c_int, c_size_t, c_uint64, c_void_p
 
 import numpy as np
@@ -192,15 +192,15 @@ def load():
     lib.wkf_q4_free.restype = None
     lib.wkf_q4_shape.argtypes = [c_void_p, POINTER(c_size_t), POINTER(c_size_t), POINTER(c_size_t)]
     lib.wkf_tensor_mat_mul_q4.argtypes = [c_void_p, c_void_p, POINTER(c_void_p)]
-    lib.wkf_tensor_norm_rope.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_float, POINTER(c_size_t), POINTER(c_void_p)]
+    lib.wkf_tensor_norm_rope.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p, c_float, c_void_p, POINTER(c_void_p)]
     lib.wkf_kv_cache_create.argtypes = [c_void_p, c_size_t, c_size_t, c_size_t, c_size_t, c_size_t, POINTER(c_void_p)]
     lib.wkf_kv_cache_free.argtypes = [c_void_p]
     lib.wkf_kv_cache_free.restype = None
     lib.wkf_kv_cache_length.argtypes = [c_void_p, c_size_t, POINTER(c_size_t)]
     lib.wkf_kv_cache_reset.argtypes = [c_void_p, c_size_t]
-    lib.wkf_kv_cache_append.argtypes = [c_void_p, c_void_p, c_void_p, POINTER(c_size_t)]
+    lib.wkf_kv_cache_append.argtypes = [c_void_p, c_void_p, c_void_p, c_void_p]
     lib.wkf_kv_cache_values.argtypes = [c_void_p, c_int, c_size_t, c_size_t, POINTER(c_void_p)]
-    lib.wkf_tensor_attend.argtypes = [c_void_p, c_void_p, c_float, c_int, POINTER(c_size_t), POINTER(c_void_p)]
+    lib.wkf_tensor_attend.argtypes = [c_void_p, c_void_p, c_float, c_int, c_void_p, POINTER(c_void_p)]
     _lib = lib
     return lib
 
@@ -213,6 +213,14 @@ def _check(rc):
 def _sizes(values):
     values = [int(v) for v in values]
     return (c_size_t * max(1, len(values)))(*values)
+
+
+def _whole(values):
+    """Whole numbers as an array of size_t, None where one is negative; a ctypes array of many costs more than a launch."""
+    try:
+        return array("Q", values)
+    except OverflowError:
+        return None
 
 
 _NP = {F32: np.float32, F16: np.float16}
@@ -658,11 +666,11 @@ class Tensor:
             if self._batch is None:  # a tensor's shape never changes
                 shape = self.shape()
                 self._batch = shape[0] if len(shape) == 4 else 1
-            if len(positions) != self._batch or min(positions, default=0) < 0:
+            positions = _whole(positions)
+            if positions is None or len(positions) != self._batch:
                 raise WkfError(ERR_INVALID_ARG, "norm_rope: one position per batch entry is required")
-            positions = (c_size_t * len(positions))(*map(operator.index, positions))
         h = c_void_p()
-        _check(self._lib.wkf_tensor_norm_rope(self._h, weight._h, cos._h, sin._h, float(eps), positions, byref(h)))
+        _check(self._lib.wkf_tensor_norm_rope(self._h, weight._h, cos._h, sin._h, float(eps), positions.buffer_info()[0] if positions else None, byref(h)))
         return self._new(h)
 
     def attend(self, cache, scale=None, causal=True, counts=None):
@@ -670,7 +678,8 @@ class Tensor:
         scale: 1 / sqrt(dim) when None.  wkf_tensor_attend."""
         h = c_void_p()
         scale = cache.head_dim ** -0.5 if scale is None else float(scale)
-        _check(self._lib.wkf_tensor_attend(self._h, cache._h, scale, 1 if causal else 0, cache._counts(counts), byref(h)))
+        counts = cache._counts(counts)
+        _check(self._lib.wkf_tensor_attend(self._h, cache._h, scale, 1 if causal else 0, counts.buffer_info()[0] if counts else None, byref(h)))
         return self._new(h)
 
     # -- data that stays on the device ----------------------------------------------
@@ -809,9 +818,10 @@ class KvCache:
     def _counts(self, counts):
         if counts is None:
             return None
-        if len(counts) != self.sequences or min(counts) < 0:
+        counts = _whole(counts)
+        if counts is None or len(counts) != self.sequences:
             raise WkfError(ERR_INVALID_ARG, "one count per sequence is required")
-        return (c_size_t * len(counts))(*map(operator.index, counts))
+        return counts
 
     def lengths(self):
         out, n = [], c_size_t()
@@ -829,7 +839,8 @@ class KvCache:
     def append(self, k, v, counts=None):
         """Stores the first counts[b] (None: all) of the tokens in k and v [sequences, kv_heads, S, head_dim] behind each
         sequence.  Runs at once: wkf_kv_cache_append."""
-        _check(self._lib.wkf_kv_cache_append(self._h, k._h, v._h, self._counts(counts)))
+        counts = self._counts(counts)
+        _check(self._lib.wkf_kv_cache_append(self._h, k._h, v._h, counts.buffer_info()[0] if counts else None))
 
     def values(self, first=0, count=None, dtype=F32):
         """What is stored for tokens first .. first + count (None: up to the longest sequence): a lazy tensor

@@ -57,11 +57,26 @@ char* ptr(const BufRef& b) { return static_cast<char*>(wkf_buffer_ptr(b.get()));
 // "name=value name=value ...": a launch's detail (a stream costs more than the launch's other host work)
 std::string detail(std::initializer_list<std::pair<const char*, size_t>> list) {
   std::string s;
+  s.reserve(96);
   for (const auto& p : list) s.append(s.empty() ? "" : " ").append(p.first).append("=").append(std::to_string(p.second));
   return s;
 }
 // the first element of a tensor's layout
 char* first(const TensorData& t) { return ptr(t.buffer) + t.layout.offset * dtype_size(t.dtype); }
+
+// texts and numbers after each other
+struct Piece {
+  const char* text;
+  size_t number = 0;
+  Piece(const char* t) : text(t) {}
+  Piece(size_t n) : text(nullptr), number(n) {}
+};
+std::string joined(std::initializer_list<Piece> list) {
+  std::string s;
+  s.reserve(96);
+  for (const Piece& p : list) p.text ? s.append(p.text) : s.append(std::to_string(p.number));
+  return s;
+}
 
 std::string define(const char* name, size_t v) { return std::string("#define ") + name + " " + std::to_string(v) + "\n"; }
 
@@ -78,7 +93,7 @@ std::string kv_defines(const KvCache& c, DType dt, size_t nb) {
   return define("WKF_H", dt == DType::F16) + define("D", c.dim) + define("DP", c.dp) + define("T", c.block) + define("NB", nb);
 }
 std::string kv_signature(const char* what, const KvCache& c, DType dt, size_t nb) {
-  return std::string(what) + "|gfx950|" + dtype_name(dt) + "|d" + std::to_string(c.dim) + "|t" + std::to_string(c.block) + "|nb" + std::to_string(nb);
+  return joined({what, "|gfx950|", dtype_name(dt), "|d", c.dim, "|t", c.block, "|nb", nb});
 }
 }  // namespace
 
@@ -123,8 +138,8 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
   int shift = -1;
   for (int i = 0; i < 32; i++)
     if (units == size_t(1) << i) shift = i;
-  const std::string kind = std::string(dtype_name(x.dtype)) + "|s" + dtype_name(w.scale_dtype) + (z ? "|zeros" : "") + "|step" + std::to_string(step) + (shift < 0 ? "|any" : "");
-  const std::string defines = define("WKF_H", h) + define("WKF_SH", w.scale_dtype == DType::F16) + define("WKF_Z", z) + define("STEP", step) + define("POW2", shift >= 0);
+  const std::string kind = joined({dtype_name(x.dtype), "|s", dtype_name(w.scale_dtype), z ? "|zeros" : "", "|step", step, shift < 0 ? "|any" : ""});
+  auto defines = [&] { return define("WKF_H", h) + define("WKF_SH", w.scale_dtype == DType::F16) + define("WKF_Z", z) + define("STEP", step) + define("POW2", shift >= 0); };
   const std::string d = detail({{"m", M}, {"n", N}, {"k", w.k}, {"group", w.group}});
   // More than 16 rows share x in the LDS; up to 32 beside few columns do not pay for it (24 rows of [4096,4096]: 9.5 us against 12.4).
   if (M > (w.tiles_n() <= 256 ? 32 : 16)) {
@@ -145,7 +160,7 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
     if (!h || w.k % 8 || reinterpret_cast<uintptr_t>(rows) % 16) {
       const size_t pieces = M * (Kp / 8);
       planes = alloc({size_t(h ? 1 : 3), M, Kp}, DType::F16, false);
-      const std::string rsig = std::string("q4_rows|gfx950|") + dtype_name(x.dtype);
+      const std::string rsig = joined({"q4_rows|gfx950|", dtype_name(x.dtype)});
       wkf_kernel* rk = kernel(rsig, [&] { return std::string(kPrelude) + define("WKF_H", h) + kQ4Rows; });
       struct {
         const void* x;
@@ -155,9 +170,9 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
       launch("q4_rows", rsig, d, rk, grid_dim((pieces + 255) / 256, "mat_mul_q4"), 1, 1, 256, ra);
       rows = ptr(planes.buffer);
     }
-    const std::string sig = "q4_tile|gfx950|" + kind + "|" + std::to_string(mt) + "x" + std::to_string(nt) + "x" + std::to_string(nw) + "x" + std::to_string(kw);
+    const std::string sig = joined({"q4_tile|gfx950|", kind.c_str(), "|", mt, "x", nt, "x", nw, "x", kw});
     wkf_kernel* k = kernel(sig, [&] {
-      return std::string(kPrelude) + defines + define("MT", mt) + define("NT", nt) + define("NW", nw) + define("KW", kw) + define("DEPTH", depth) + kQ4Numbers + kQ4Tile;
+      return std::string(kPrelude) + defines() + define("MT", mt) + define("NT", nt) + define("NW", nw) + define("KW", kw) + define("DEPTH", depth) + kQ4Numbers + kQ4Tile;
     });
     struct {
       const void *x, *codes, *scales, *zeros;
@@ -171,9 +186,9 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
   const size_t mt = M <= 16 ? 1 : 2;
   // eight waves, two tiles each on their way ([1,4096]x[4096,11008] f16: 9.0 us, 10.7 with four waves, 10.0 with sixteen, 10.8 with four tiles)
   constexpr size_t waves = 8, pf = 2;
-  const std::string sig = "q4_mat_mul|gfx950|" + kind + "|w" + std::to_string(waves) + "|pf" + std::to_string(pf) + "|mt" + std::to_string(mt);
+  const std::string sig = joined({"q4_mat_mul|gfx950|", kind.c_str(), "|w", waves, "|pf", pf, "|mt", mt});
   wkf_kernel* k = kernel(sig, [&] {
-    return std::string(kPrelude) + defines + define("WAVES", waves) + define("PF", pf) + define("MT", mt) + kQ4Numbers + kQ4MatMul;
+    return std::string(kPrelude) + defines() + define("WAVES", waves) + define("PF", pf) + define("MT", mt) + kQ4Numbers + kQ4MatMul;
   });
   struct {
     const void *x, *codes, *scales, *zeros;
@@ -251,7 +266,7 @@ size_t nr_dim(const Node* n, size_t i) {
 namespace {
 // whether the value of `n` is computed from that of `from`
 bool depends(const NodeP& n, const Node* from, std::set<const Node*>* seen) {
-  if (!n || !seen->insert(n.get()).second) return false;
+  if (!n || n->kind == NodeKind::Tensor || !seen->insert(n.get()).second) return false;
   if (n.get() == from) return true;
   for (const NodeP& m : n->more)
     if (depends(m, from, seen)) return true;
@@ -316,8 +331,7 @@ std::vector<TensorData> Resolver::launch_norm_rope(const std::vector<const Node*
   size_t v = n0->dtype == DType::F16 ? 8 : 4, lanes = 1;
   while (dim / 2 % v) v /= 2;
   while (lanes < 64 && lanes * v < dim / 2) lanes *= 2;
-  const std::string sig = std::string("norm_rope|gfx950|") + dtype_name(n0->dtype) + "|w" + dtype_name(ws[0].dtype) + "|t" + dtype_name(cos.dtype) + "|d" + std::to_string(dim) +
-                          (full ? "|full" : "") + "|nb" + std::to_string(nb) + "|x" + std::to_string(count);
+  const std::string sig = joined({"norm_rope|gfx950|", dtype_name(n0->dtype), "|w", dtype_name(ws[0].dtype), "|t", dtype_name(cos.dtype), "|d", dim, full ? "|full" : "", "|nb", nb, "|x", count});
   wkf_kernel* k = kernel(sig, [&] {
     return std::string(kPrelude) + define("WKF_H", n0->dtype == DType::F16) + define("WKF_WH", ws[0].dtype == DType::F16) + define("WKF_TH", cos.dtype == DType::F16) +
            define("D", dim) + define("FULL", full) + define("V", v) + define("LANES", lanes) + define("NB", nb) + define("MEMBERS", count) + kNormRope;
@@ -327,6 +341,7 @@ std::vector<TensorData> Resolver::launch_norm_rope(const std::vector<const Node*
     const size_t bn = std::min(batch - b0, kMaxSequences);
     // Member[count], then cos, sin, seq, batch, heads, eps, positions[nb]: kernels/norm_rope.hip.inc
     std::vector<unsigned char> block;
+    block.reserve(count * 64 + 64 + nb * 4);
     auto put = [&](const void* p, size_t bytes) { block.insert(block.end(), static_cast<const unsigned char*>(p), static_cast<const unsigned char*>(p) + bytes); };
     for (size_t i = 0; i < count; i++) {
       const Layout& l = xs[i].layout;

@@ -167,6 +167,7 @@ class Resolver {
   // sibling norm_rope roots (the heads of q and of k) as one launch; leaves their values in materialized_
   void join_norm_ropes(const std::vector<NodeP>& roots);
   std::vector<TensorData> launch_norm_rope(const std::vector<const Node*>& members);
+  bool resolve_flat(const std::vector<NodeP>& roots, const std::vector<TensorData>& outs);
   TensorData rows_dense(const NodeP& n);
   TensorData result_of(const Node* n);
   void copy_map(const TensorData& from, const TensorData& to);
