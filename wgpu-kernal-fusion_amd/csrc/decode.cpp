@@ -129,10 +129,12 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
   if (!M) return out;
   if (M > 0xfffffull) throw Error(WKF_ERR_UNSUPPORTED, "mat_mul_q4: more than 2^20 rows");
   const bool z = bool(w.zeros), h = x.dtype == DType::F16;
-  // Many f16 rows: the weights are written out once, each rounded to f16, and the product is mat_mul's ([1024,4096]x[4096,11008]:
-  // 112 us against 153 in tiles of 4-bit weights, 512 rows 74 against 78, 512 rows of [4096,4096] 42 against 27).  Weights that
-  // would overflow or lose bits there stay in the tiles, which round none.
-  if (h && w.fits_f16 && M >= 768 && N >= 16 && w.tiles_n() <= 65535 && M * N * Kp >= (size_t(1) << 18)) return mat_mul_q4_dense(w, x, out, M);
+  auto tiles_of = [&](size_t mt, size_t columns) { return (M + 16 * mt - 1) / (16 * mt) * ((w.tiles_n() + columns - 1) / columns); };
+  // Many f16 rows: where no tiles below cover the product with one round of the chip, the weights are written out once, each
+  // rounded to f16, and the product is mat_mul's ([1024,4096]x[4096,11008]: 114 us against 122 in tiles of 4-bit weights;
+  // [1024,11008]x[11008,4096], which one round covers: 154 against 104).  Weights that would overflow or lose bits in f16
+  // stay in the tiles, which round none.
+  if (h && w.fits_f16 && M >= 768 && tiles_of(4, 32) > 256 && w.tiles_n() <= 65535) return mat_mul_q4_dense(w, x, out, M);
   // the k = 32 steps of a tile that surely share a group, and the group in units of so many
   const size_t step = w.group % 128 == 0 ? 4 : w.group % 64 == 0 ? 2 : 1, units = w.group / (32 * step);
   int shift = -1;
@@ -143,18 +145,17 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
   const std::string d = detail({{"m", M}, {"n", N}, {"k", w.k}, {"group", w.group}});
   // More than 16 rows share x in the LDS; up to 32 beside few columns do not pay for it (24 rows of [4096,4096]: 9.5 us against 12.4).
   if (M > (w.tiles_n() <= 256 ? 32 : 16)) {
-    // Tiles of 32 rows x 64 columns with K shared by as many groups of waves as the LDS has room for, until there are more of
-    // them than the chip takes at once; then larger ones, which read x less often ([4096,4096] f16: 128 rows 14.6 us against 26
-    // in tiles of 64 x 128, 256 rows 27.6 against 24; f32 256 rows 48 in 32 x 128 against 68 and 108, 1024 rows 116 in 64 x 256).
-    size_t mt = 2, nt = 1, nw = 4, kw = h ? 4 : 2;
+    // The smallest tiles of which the chip takes all at once, one a compute unit: larger ones read x less often, smaller ones
+    // have K shared by more groups of waves ([4096,4096] f16: 256 rows 19.7 us in 32 x 128, 28.7 in 32 x 64, 28.3 in 64 x 128;
+    // 1024 rows 42 in 64 x 256, 54 in 64 x 128; f32 256 rows 46 in 32 x 128, 70 in 32 x 64, 67 in 32 x 256).
+    struct Tile {
+      size_t mt, nt, nw, kw;
+    };
+    static constexpr Tile f16_tiles[] = {{2, 1, 4, 4}, {2, 2, 4, 4}, {4, 2, 4, 2}, {4, 2, 8, 1}, {4, 4, 8, 1}}, f32_tiles[] = {{2, 1, 4, 2}, {2, 1, 8, 2}, {2, 2, 8, 1}};
+    const Tile *tile = h ? f16_tiles : f32_tiles, *last = h ? std::end(f16_tiles) - 1 : std::end(f32_tiles) - 1;
+    while (tile < last && tiles_of(tile->mt, tile->nt * tile->nw) > 256) tile++;
+    const size_t mt = tile->mt, nt = tile->nt, nw = tile->nw, kw = tile->kw;
     constexpr size_t depth = 2;
-    const size_t by32 = (M + 31) / 32;
-    if (h) {
-      if (by32 * ((w.tiles_n() + 3) / 4) > 512) mt = 4, nt = 2, kw = 2;
-    } else if (by32 * ((w.tiles_n() + 3) / 4) > 256) {
-      nt = 2;
-      if (by32 * ((w.tiles_n() + 7) / 8) > 512) mt = 4, nw = 8, kw = 1;
-    }
     const void* rows = first(x);
     TensorData planes;
     if (!h || w.k % 8 || reinterpret_cast<uintptr_t>(rows) % 16) {
