@@ -285,6 +285,22 @@ def test_append_stores_what_the_definition_says(gpu, dim, block, lengths, dtype)
 
 
 @DTYPES
+@pytest.mark.parametrize("dim", [1, 66, 80, 100, 128, 255])
+def test_values_of_windows(gpu, dim, dtype):
+    """Windows that start and end anywhere, over the ends of sequences, are cut from the whole."""
+    w, rng = load_package(), rng_of(31, dim)
+    cache, held, _ = filled(gpu, rng, dtype, [75, 0, 131], 3, dim, 32, capacity=140)
+    windows = [(0, 140), (1, 1), (2, 5), (3, 70), (74, 2), (129, 9), (130, 1), (137, 3), (5, 0)]
+    got = computed(*[cache.values(at, n, w.F16 if dtype == F16 else w.F32) for at, n in windows])
+    want = np.zeros((2, 3, 3, 140, dim))
+    for b in range(3):
+        for kv in range(2):
+            want[kv, b, :, :held[b][kv].shape[1]] = held[b][kv]
+    for g, (at, n) in zip(got, windows):
+        assert g.shape == (2, 3, 3, n, dim) and np.array_equal(g, want[:, :, :, at:at + n].astype(F32).astype(dtype))
+
+
+@DTYPES
 def test_append_in_pieces_gives_the_cache_of_one_append(gpu, dtype):
     """Tokens one at a time, in pieces that end inside a block, on its border and across several, by sequences of their own pace."""
     w, rng = load_package(), rng_of(31)

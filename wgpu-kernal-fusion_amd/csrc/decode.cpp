@@ -497,7 +497,9 @@ TensorData Resolver::run_cache_values(const NodeP& n) {
   if (!args.count) return out;
   const size_t nb = room_for(c.seqs);
   const std::string sig = kv_signature("kv_values", c, n->dtype, nb);
-  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + kv_defines(c, n->dtype, nb) + kKvLayout + kKvValues; });
+  size_t v = n->dtype == DType::F16 ? 8 : 4;
+  while (c.dim % v) v /= 2;
+  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + define("V", v) + kv_defines(c, n->dtype, nb) + kKvLayout + kKvValues; });
   with_room<ValuesArgs>(nb, [&](auto& a) {
     a.out = first(out);
     a.codes = ptr(c.codes);
@@ -508,7 +510,8 @@ TensorData Resolver::run_cache_values(const NodeP& n) {
     a.first = uint32_t(args.first);
     a.count = uint32_t(args.count);
     std::copy(c.len.begin(), c.len.end(), a.len);
-    launch("kv_values", sig, "tokens=" + std::to_string(args.count), k, grid_dim((args.count + 15) / 16, "kv_cache_values"), uint32_t(c.heads), uint32_t(2 * c.seqs), 256, a);
+    const size_t fours = (args.first + args.count + 3) / 4 - args.first / 4, threads = fours * (c.dim / v);
+    launch("kv_values", sig, "tokens=" + std::to_string(args.count), k, grid_dim((threads + 255) / 256, "kv_cache_values"), uint32_t(c.heads), uint32_t(2 * c.seqs), 256, a);
   });
   return out;
 }
@@ -524,7 +527,7 @@ TensorData Resolver::run_attend(const NodeP& n) {
   if (!out.layout.numel()) return out;
   const size_t nb = room_for(c.seqs), share = heads / c.heads, tiles = (share * rows + 15) / 16;
   // Rows enough to give every compute unit a tile of 128: the kernel that spreads the codes in the LDS for all of them
-  // (2048 new tokens after 2048, 32/8 heads: 512 tiles, 133 us against 276 in tiles of 16 rows).  With fewer tiles the cache has
+  // (2048 new tokens after 2048, 32/8 heads: 512 tiles, 121 us against 276 in tiles of 16 rows).  With fewer tiles the cache has
   // to be split over workgroups, which the kernel for tiles of 16 rows does (512 new tokens after 3584: 101 us against 89).
   const size_t big = (share * rows + 127) / 128;
   if (share * rows > 64 && big * c.heads * c.seqs >= 256) {
@@ -555,9 +558,10 @@ TensorData Resolver::run_attend(const NodeP& n) {
   }
   // How many groups of 32 tokens a workgroup takes: so few that there are nearly as many workgroups as the chip holds at once
   // (512; large heads leave registers for 256), and no more, where a second round would begin (16 sequences of 17000 to 32768
-  // tokens, 8 key heads: 149 us, against 174 with 304 workgroups; 8 sequences of up to 3000, 8 heads of 256: 26 us, 33 with 512).  Joining s parts costs about as much as reading s groups, so a few long sequences
-  // are split no finer than the square root of twice their groups (one sequence, 8 key heads: 4000 tokens 16.6 us in 32 parts,
-  // 11.9 in 8; 16000 tokens 21.4 us in 32 parts, 19.3 in 16).  Up to 16 groups stay whole: the join alone takes 3 us.
+  // tokens, 8 key heads: 149 us, against 174 with 304 workgroups; 8 sequences of up to 3000, 8 heads of 256: 26 us, 33 with
+  // 512).  Joining s parts costs about as much as reading s groups, so a few long sequences are split no finer than the square
+  // root of twice their groups (one sequence, 8 key heads: 4000 tokens 16.6 us in 32 parts, 11.9 in 8; 16000 tokens 21.4 us in 32
+  // parts, 19.3 in 16).  Up to 16 groups stay whole: the join alone takes 3 us.
   size_t total = 0, longest = 0;
   for (uint32_t n : c.len) {
     total += (n + 31) / 32;
