@@ -312,16 +312,34 @@ std::vector<TensorData> Resolver::launch_norm_rope(const std::vector<const Node*
   const Node* n0 = members[0];
   const NormRopeArgs& args = norm_rope_args(n0);
   const size_t batch = nr_dim(n0, 0), seq = nr_dim(n0, 2), dim = nr_dim(n0, 3);
-  auto dense = [&](const NodeP& n) {
-    TensorData t = resolve(n);
-    return t.layout.strides == Layout::contiguous_strides(t.layout.shape) ? t : make_contiguous(t);
+  // an input's value with the last `dims` dimensions dense; a leaf's own is not copied
+  TensorData kept[2 + 2 * kMaxMembers];
+  size_t used = 0;
+  auto value = [&](const NodeP& n, size_t dims) {
+    const TensorData* t = &n->data;
+    TensorData& own = kept[used++];
+    if (n->kind != NodeKind::Tensor) {
+      own = resolve(n);
+      t = &own;
+    }
+    size_t want = 1;
+    for (size_t i = t->layout.rank(), k = 0; i-- && k < dims; k++) {
+      if (t->layout.shape[i] > 1 && t->layout.strides[i] != want) {
+        own = make_contiguous(*t);
+        return const_cast<const TensorData*>(&own);
+      }
+      want *= t->layout.shape[i];
+    }
+    return t;
   };
-  TensorData cos = dense(n0->more[1]), sin = dense(n0->more[2]);
-  std::vector<TensorData> xs, ws, outs;
+  const TensorData &cos = *value(n0->more[1], 2), &sin = *value(n0->more[2], 2);
+  const TensorData *xs[kMaxMembers], *ws[kMaxMembers];
+  std::vector<TensorData> outs;
+  outs.reserve(members.size());
   size_t heads = 0;
   for (const Node* n : members) {
-    xs.push_back(rows_dense(n->a));
-    ws.push_back(dense(n->more[0]));
+    xs[outs.size()] = value(n->a, 1);
+    ws[outs.size()] = value(n->more[0], 1);
     outs.push_back(result_of(n));
     heads += nr_dim(n, 1);
   }
@@ -332,9 +350,9 @@ std::vector<TensorData> Resolver::launch_norm_rope(const std::vector<const Node*
   size_t v = n0->dtype == DType::F16 ? 8 : 4, lanes = 1;
   while (dim / 2 % v) v /= 2;
   while (lanes < 64 && lanes * v < dim / 2) lanes *= 2;
-  const std::string sig = joined({"norm_rope|gfx950|", dtype_name(n0->dtype), "|w", dtype_name(ws[0].dtype), "|t", dtype_name(cos.dtype), "|d", dim, full ? "|full" : "", "|nb", nb, "|x", count});
+  const std::string sig = joined({"norm_rope|gfx950|", dtype_name(n0->dtype), "|w", dtype_name(ws[0]->dtype), "|t", dtype_name(cos.dtype), "|d", dim, full ? "|full" : "", "|nb", nb, "|x", count});
   wkf_kernel* k = kernel(sig, [&] {
-    return std::string(kPrelude) + define("WKF_H", n0->dtype == DType::F16) + define("WKF_WH", ws[0].dtype == DType::F16) + define("WKF_TH", cos.dtype == DType::F16) +
+    return std::string(kPrelude) + define("WKF_H", n0->dtype == DType::F16) + define("WKF_WH", ws[0]->dtype == DType::F16) + define("WKF_TH", cos.dtype == DType::F16) +
            define("D", dim) + define("FULL", full) + define("V", v) + define("LANES", lanes) + define("NB", nb) + define("MEMBERS", count) + kNormRope;
   });
   const size_t e = dtype_size(n0->dtype);
@@ -345,13 +363,13 @@ std::vector<TensorData> Resolver::launch_norm_rope(const std::vector<const Node*
     block.reserve(count * 64 + 64 + nb * 4);
     auto put = [&](const void* p, size_t bytes) { block.insert(block.end(), static_cast<const unsigned char*>(p), static_cast<const unsigned char*>(p) + bytes); };
     for (size_t i = 0; i < count; i++) {
-      const Layout& l = xs[i].layout;
+      const Layout& l = xs[i]->layout;
       const size_t r = l.rank(), hn = nr_dim(members[i], 1);
       struct {
         const void *x, *y, *w;
         uint64_t sb, sh, ss, yb;
         uint32_t heads, pad;
-      } m = {first(xs[i]) + (r == 4 ? b0 * l.strides[0] * e : 0), first(outs[i]) + b0 * hn * seq * dim * e, first(ws[i]),
+      } m = {first(*xs[i]) + (r == 4 ? b0 * l.strides[0] * e : 0), first(outs[i]) + b0 * hn * seq * dim * e, first(*ws[i]),
              r == 4 ? l.strides[0] : 0, l.strides[r - 3], l.strides[r - 2], hn * seq * dim, uint32_t(hn), 0};
       put(&m, sizeof(m));
     }
