@@ -1,5 +1,7 @@
 """The decoder operators on the GPU against their plain forms in 64 bits (tests/decode_reference.py): sizes and masks
 where they can go wrong, strided inputs, both element types, and a run of them together."""
+from concurrent.futures import ThreadPoolExecutor
+
 import numpy as np
 import pytest
 
@@ -642,6 +644,37 @@ def test_a_block_serves_a_prompt_and_then_tokens(gpu, dtype):
     if gpu.is_planner:
         pytest.skip("plan-only device: kernels compiled, nothing computed")
     assert cache.lengths() == lengths
+
+
+def test_two_threads_at_once(gpu):
+    """Two programs on one device, weights shared, a cache each, and one cache that both read: the values of one after the other."""
+    w, rng = load_package(), rng_of(47)
+    codes, scales, z = ref.q4_weights(rng, 256, 256, 64, True, F16)
+    weights = w.Q4Weights(gpu, codes, scales, z, 64)
+    x = rng.standard_normal((2, 20, 256)).astype(F16)
+    common = w.KvCache(gpu, 1, 2, 64, 3000, 64)
+    k = rng.standard_normal((1, 2, 3000, 64)).astype(F16)
+    common.append(leaf(gpu, k), leaf(gpu, k))
+
+    def program(i):
+        cache, out, seen = w.KvCache(gpu, 1, 2, 64, 400, 32), w.Tensor.zeros(gpu, (1, 4, 20, 64), w.F16), []
+        t = leaf(gpu, x[i])
+        for _ in range(12):
+            y = t.mat_mul_q4(weights)
+            heads = y.reshape([20, 4, 64]).transpose(0, 1).reshape([1, 4, 20, 64])
+            cache.append(heads.narrow(1, 0, 2), heads.narrow(1, 2, 2))
+            w.materialize_into([heads.attend(cache) + heads.attend(common)], [out])
+            seen.append(None if gpu.is_planner else out.to_numpy())
+        return seen
+
+    alone = [program(0), program(1)]
+    if gpu.is_planner:
+        pytest.skip("plan-only device: kernels compiled, nothing computed")
+    with ThreadPoolExecutor(2) as pool:
+        both = list(pool.map(program, range(2)))
+    for one, other in zip(alone, both):
+        assert all(np.array_equal(a, b) for a, b in zip(one, other))
+        assert np.isfinite(one[-1]).all() and not np.array_equal(one[0], one[-1])
 
 
 def test_views_of_device_memory(gpu):

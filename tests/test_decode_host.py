@@ -106,6 +106,8 @@ def test_refusals_of_weights_in_4_bits(wkf, planner):
         zeros(wkf, planner, ()).mat_mul_q4(w)
     with refused(wkf, "different devices"):
         zeros(wkf, wkf.Device.planner(), (3, 64)).mat_mul_q4(w)
+    with refused(wkf, "more than 2.20 - 1 rows"):
+        zeros(wkf, planner, (1, 64), F16).reshape([64]).broadcast(((1 << 20), 64)).mat_mul_q4(w).materialize()
     y = zeros(wkf, planner, (2, 3, 64), F16).mat_mul_q4(w)
     assert y.shape() == (2, 3, 16) and y.datatype() == wkf.F16
     assert zeros(wkf, planner, (64,)).mat_mul_q4(w).shape() == (16,)

@@ -127,7 +127,7 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
   TensorData out = result_of(n.get());
   const size_t M = x.layout.numel() / w.k, N = w.n, Kp = (w.k + 7) / 8 * 8;
   if (!M) return out;
-  if (M > 0xfffffull) throw Error(WKF_ERR_UNSUPPORTED, "mat_mul_q4: more than 2^20 rows");
+  if (M > 0xfffffull) throw Error(WKF_ERR_UNSUPPORTED, "mat_mul_q4: more than 2^20 - 1 rows");
   const bool z = bool(w.zeros), h = x.dtype == DType::F16;
   auto tiles_of = [&](size_t mt, size_t columns) { return (M + 16 * mt - 1) / (16 * mt) * ((w.tiles_n() + columns - 1) / columns); };
   // Many f16 rows: where no tiles below cover the product with one round of the chip, the weights are written out once, each
