@@ -99,6 +99,44 @@ def test_mat_mul_q4(gpu, case, dtype):
     ref.close(got, x.astype(np.float64) @ dense, dtype, ref.q4_slack(x, dense, q4_rounds_weights(dtype, m)), str(case))
 
 
+Q4_PATHS = [  # dtype, m, k, n, group, zeros, scale dtype, what the kernel's signature has
+    (F16, 16, 200, 70, 32, True, F16, "q4_mat_mul|gfx950|f16|sf16|zeros|step1|w8|pf2|mt1"), (F16, 24, 264, 300, 64, False, F32, "|mt2"), (F32, 24, 264, 300, 64, False, F32, "|mt2"),
+    (F16, 33, 296, 200, 128, True, F16, "|2x1x4x4"), (F16, 300, 160, 2000, 64, False, F16, "|2x2x4x4"), (F16, 600, 1031, 2000, 96, True, F32, "|4x2x4x2"),
+    (F16, 1100, 130, 2000, 128, True, F16, "|4x2x8x1"), (F16, 600, 203, 7000, 32, True, F16, "|4x4x8x1"),
+    (F16, 1100, 130, 7700, 128, True, F16, "q4_dense"), (F16, 800, 72, 11001, 32, False, F32, "q4_dense"),
+    (F32, 33, 296, 200, 128, True, F16, "|2x1x4x2"), (F32, 300, 1031, 2000, 96, True, F32, "|2x1x8x2"), (F32, 600, 203, 2000, 64, False, F16, "|2x2x8x1"),
+]
+
+
+@pytest.mark.parametrize("case", Q4_PATHS, ids=lambda c: f"{c[0].__name__}-{c[1]}x{c[2]}x{c[3]}")
+def test_mat_mul_q4_by_every_kernel(gpu, case):
+    """A dense x and one whose rows start anywhere, a result of its own and one written where it is wanted, infinities and
+    NaN that stay in their rows."""
+    w, (dtype, m, k, n, group, zeros, sdt, kernel) = load_package(), case
+    rng = rng_of(17, m, k, n, group)
+    codes, scales, z = ref.q4_weights(rng, k, n, group, zeros, sdt)
+    weights, dense = w.Q4Weights(gpu, codes, scales, z, group), ref.q4_dense(codes, scales, z, group)
+    x = rng.standard_normal((m, k)).astype(dtype)
+    odd = {1: np.nan, 5: np.inf, m - 1: -np.inf}
+    for row, v in odd.items():
+        x[row, row % k] = v
+    flat = np.concatenate([np.zeros(3, dtype), x.reshape(-1)])
+    first, second = leaf(gpu, x).mat_mul_q4(weights), leaf(gpu, flat).narrow(0, 3, m * k).reshape([m, k]).mat_mul_q4(weights)
+    out = w.Tensor.zeros(gpu, (m, n), w.F16 if dtype == F16 else w.F32)
+    first.materialize()
+    assert any(kernel in i.signature for i in first.kernels()), [i.signature for i in first.kernels()]
+    w.materialize_into([second], [out])
+    got, placed = computed(first, out)
+    finite = np.where(np.isfinite(x), x, 0).astype(np.float64)
+    want = finite @ dense
+    for row in odd:
+        with np.errstate(invalid="ignore"):
+            want[row] = (x[row].astype(np.float64)[:, None] * dense).sum(0)
+    slack = ref.q4_slack(finite, dense, q4_rounds_weights(dtype, m))
+    ref.close(got, want, dtype, slack)
+    ref.close(placed, want, dtype, slack)
+
+
 @DTYPES
 def test_mat_mul_q4_of_views_batches_and_expressions(gpu, dtype):
     w, rng = load_package(), rng_of(11)
@@ -163,11 +201,14 @@ def test_mat_mul_q4_with_scales_that_are_not_finite(gpu):
 def test_mat_mul_q4_of_weights_beyond_f16(gpu, scale):
     """Weights that f16 could not hold, or not with all its bits, meet many rows of f16."""
     w, rng = load_package(), rng_of(16)
-    codes, scales, z = ref.q4_weights(rng, 96, 40, 32, True, F32)
+    codes, scales, z = ref.q4_weights(rng, 96, 11008, 32, True, F32)
     scales = (scales * F32(scale / 0.02)).astype(F32)
     x = (rng.standard_normal((800, 96)) * min(1.0, 1e-3 / scale)).astype(F16)
     dense = ref.q4_dense(codes, scales, z, 32)
-    ref.close(computed(leaf(gpu, x).mat_mul_q4(w.Q4Weights(gpu, codes, scales, z, 32))), x.astype(np.float64) @ dense, F16, ref.q4_slack(x, dense))
+    y = leaf(gpu, x).mat_mul_q4(w.Q4Weights(gpu, codes, scales, z, 32))
+    y.materialize()
+    assert not any("q4_dense" in i.signature for i in y.kernels())
+    ref.close(computed(y), x.astype(np.float64) @ dense, F16, ref.q4_slack(x, dense))
 
 
 def test_mat_mul_q4_without_rows(gpu):
