@@ -197,7 +197,7 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
     uint32_t m, n, k, group, groups, tiles_k, shift, pad;
   } a = {first(x), ptr(w.codes), ptr(w.scales), z ? ptr(w.zeros) : nullptr, first(out),
          uint32_t(M), uint32_t(N), uint32_t(w.k), uint32_t(w.group), uint32_t(w.groups), uint32_t(w.tiles_k()), uint32_t(std::max(shift, 0)), 0};
-  launch("q4_mat_mul", sig, d, k, uint32_t(w.tiles_n()), uint32_t((M + 16 * mt - 1) / (16 * mt)), 1, uint32_t(64 * waves), a);
+  launch("q4_mat_mul", sig, d, k, grid_dim(w.tiles_n(), "mat_mul_q4", 64 * waves), uint32_t((M + 16 * mt - 1) / (16 * mt)), 1, uint32_t(64 * waves), a);
   return out;
 }
 
