@@ -211,6 +211,37 @@ def test_mat_mul_q4_of_weights_beyond_f16(gpu, scale):
     ref.close(computed(y), x.astype(np.float64) @ dense, F16, ref.q4_slack(x, dense))
 
 
+Q4_LARGE = [(1, 200, 70, 32, True, "q4_mat_mul"), (7, 384, 40, 128, False, "q4_mat_mul"), (24, 200, 300, 64, True, "|mt2"), (33, 296, 200, 128, True, "|2x1x4x2"),
+            (300, 330, 2000, 96, False, "|2x1x8x2"), (600, 203, 2000, 32, True, "|2x2x8x1")]
+
+
+@pytest.mark.parametrize("case", Q4_LARGE, ids=lambda c: "x".join(str(v) for v in c[:4]))
+def test_mat_mul_q4_of_the_largest_numbers(gpu, case):
+    """Rows near f32's largest number and scales far below 1: x times codes leaves f32, the product with the weights does not.
+    Rows of an ordinary size beside them, and one with an infinity, are what they are alone."""
+    w, (m, k, n, group, zeros, kernel) = load_package(), case
+    rng = rng_of(18, m, k, n, group)
+    codes, scales, z = ref.q4_weights(rng, k, n, group, zeros, F32)
+    scales = (scales * F32(2.0 ** -8)).astype(F32)
+    x = rng.choice([-1.0, 1.0], (m, k)) * rng.uniform(0.5, 1, (m, k)) * 3.4e38
+    x[2::3] /= 1e38
+    x = x.astype(F32)
+    if m > 1:
+        x[1] = np.abs(x[1])  # every product of a column of one sign has it
+        x[m - 1, 5] = np.inf
+    dense = ref.q4_dense(codes, scales, z, group)
+    y = leaf(gpu, x).mat_mul_q4(w.Q4Weights(gpu, codes, scales, z, group))
+    y.materialize()
+    assert any(kernel in i.signature for i in y.kernels()), [i.signature for i in y.kernels()]
+    finite = np.where(np.isfinite(x), x, 0).astype(np.float64)
+    want = finite @ dense
+    assert np.abs(want).max() < 3e38
+    if m > 1:
+        with np.errstate(invalid="ignore"):
+            want[m - 1] = (x[m - 1].astype(np.float64)[:, None] * dense).sum(0)
+    ref.close(computed(y), want, F32, ref.q4_slack(finite, dense), str(case))
+
+
 def test_mat_mul_q4_without_rows(gpu):
     w = load_package()
     codes, scales, z = ref.q4_weights(rng_of(13), 64, 20, 32, False, F16)
