@@ -113,6 +113,15 @@ def test_refusals_of_weights_in_4_bits(wkf, planner):
     assert zeros(wkf, planner, (64,)).mat_mul_q4(w).shape() == (16,)
 
 
+def test_the_shape_of_weights_is_what_they_were_made_with(wkf, planner):
+    """A group larger than the matrix too, whose length decides nothing."""
+    lib = wkf.load()
+    for k, n, group in ((64, 16, 32), (64, 16, 4096), (40, 3, 64), (1000, 100, 1024), (33, 1, 1 << 40)):
+        w, got = weights(wkf, planner, k, n, group), [ctypes.c_size_t() for _ in range(3)]
+        wkf._check(lib.wkf_q4_shape(w._h, *[ctypes.byref(v) for v in got]))
+        assert tuple(v.value for v in got) == (k, n, group)
+
+
 def test_refusals_of_norm_rope(wkf, planner):
     t, g, c = zeros(wkf, planner, (2, 3, 5, 8), F16), zeros(wkf, planner, (8,), F16), zeros(wkf, planner, (9, 4))
     ok = dict(weight=g, cos=c, sin=c, eps=1e-5)

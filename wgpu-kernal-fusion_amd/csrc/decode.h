@@ -22,7 +22,8 @@ constexpr size_t kMaxSequences = 256;
 // scales, zeros: [n/16][groups][16], the scales in their own type, a zero point a byte.
 struct Q4 {
   wkf_device* dev = nullptr;
-  size_t k = 0, n = 0, group = 0, groups = 0;
+  size_t k = 0, n = 0, group = 0, groups = 0;  // group: at most k rounded up to 32
+  size_t given_group = 0;
   DType scale_dtype = DType::F16;
   BufRef codes, scales, zeros;  // zeros: none = 8 everywhere
   bool fits_f16 = false;        // every weight is zero, or within the normal numbers of f16 when it is rounded to that

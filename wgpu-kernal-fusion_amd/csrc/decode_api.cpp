@@ -151,6 +151,7 @@ int wkf_q4_new(wkf_device* dev, size_t k, size_t n, size_t group, const void* co
     w->k = k;
     w->n = n;
     w->groups = (k + group - 1) / group;
+    w->given_group = group;
     w->group = std::min(group, (k + 31) / 32 * 32);  // one group: its length does not matter
     w->scale_dtype = dtype_of(scale_dtype, who);
     auto high = [](const void* p, size_t bytes) {
@@ -192,7 +193,7 @@ int wkf_q4_shape(const wkf_q4* w, size_t* k, size_t* n, size_t* group) {
     need(w, "wkf_q4_shape");
     if (k) *k = w->w->k;
     if (n) *n = w->w->n;
-    if (group) *group = w->w->group;
+    if (group) *group = w->w->given_group;
   });
 }
 
