@@ -14,7 +14,7 @@ class Q4Weights {
   template <class S>
   static Q4Weights make(const Device& dev, size_t k, size_t n, size_t group, const std::vector<uint8_t>& codes,
                         const std::vector<typename S::host_type>& scales, const std::vector<uint8_t>& zeros = {}) {
-    const size_t groups = group ? (k + group - 1) / group : 0;
+    const size_t groups = group ? k / group + (k % group != 0) : 0;
     if (codes.size() != k * n || scales.size() != groups * n || (!zeros.empty() && zeros.size() != groups * n))
       throw Error(WKF_ERR_INVALID_ARG, "Q4Weights: codes, scales or zeros of another size");
     wkf_q4* h = nullptr;

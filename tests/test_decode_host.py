@@ -113,6 +113,15 @@ def test_refusals_of_weights_in_4_bits(wkf, planner):
     assert zeros(wkf, planner, (64,)).mat_mul_q4(w).shape() == (16,)
 
 
+def test_a_group_of_any_size_has_scales_and_zeros(wkf, planner):
+    """k rounded up to groups is one group, however large: its zero points are looked at."""
+    lib, h = wkf.load(), ctypes.c_void_p()
+    codes, scales, zeros = np.zeros((64, 16), np.uint8), np.ones((1, 16), F16), np.full((1, 16), 16, np.uint8)
+    p = lambda a: a.ctypes.data_as(ctypes.c_void_p)  # noqa: E731
+    for group in (64, 1 << 63, (1 << 64) - 32):
+        assert lib.wkf_q4_new(planner._h, 64, 16, group, p(codes), 1, p(scales), p(zeros), ctypes.byref(h)) == wkf.ERR_INVALID_ARG
+
+
 def test_the_shape_of_weights_is_what_they_were_made_with(wkf, planner):
     """A group larger than the matrix too, whose length decides nothing."""
     lib = wkf.load()

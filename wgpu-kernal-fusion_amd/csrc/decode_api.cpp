@@ -150,7 +150,7 @@ int wkf_q4_new(wkf_device* dev, size_t k, size_t n, size_t group, const void* co
     w->dev = dev;
     w->k = k;
     w->n = n;
-    w->groups = (k + group - 1) / group;
+    w->groups = k / group + (k % group != 0);  // (k + group may pass 64 bits)
     w->given_group = group;
     w->group = std::min(group, (k + 31) / 32 * 32);  // one group: its length does not matter
     w->scale_dtype = dtype_of(scale_dtype, who);
