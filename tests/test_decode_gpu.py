@@ -242,6 +242,23 @@ def test_mat_mul_q4_of_the_largest_numbers(gpu, case):
     ref.close(computed(y), want, F32, ref.q4_slack(finite, dense), str(case))
 
 
+def test_mat_mul_q4_of_a_square_matrix_and_rows_behind_the_first_element(gpu):
+    """A copy of x has the product's shape here; the weights are written out."""
+    w, rng = load_package(), rng_of(19)
+    n, m = 6656, 1300
+    codes, scales, z = ref.q4_weights(rng, n, n, 128, True, F16)
+    flat = rng.standard_normal(m * n + 8).astype(F16)
+    t, out = leaf(gpu, flat), w.Tensor.zeros(gpu, (m, n), w.F16)
+    y = t.narrow(0, 8, m * n).reshape([m, n]).mat_mul_q4(w.Q4Weights(gpu, codes, scales, z, 128))
+    w.materialize_into([y], [out])
+    assert "q4_dense" in [i.kind for i in y.kernels()]
+    got, alone, x = *computed(out, y), flat[8:].reshape(m, n)
+    rows = np.r_[0:4, 700:704, m - 4:m]
+    dense = ref.q4_dense(codes, scales, z, 128)
+    ref.close(got[rows], x[rows].astype(np.float64) @ dense, F16, ref.q4_slack(x[rows], dense, True))
+    assert np.array_equal(got, alone) and np.array_equal(computed(t), flat)
+
+
 def test_mat_mul_q4_without_rows(gpu):
     w = load_package()
     codes, scales, z = ref.q4_weights(rng_of(13), 64, 20, 32, False, F16)

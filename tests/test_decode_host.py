@@ -263,6 +263,24 @@ def test_what_becomes_which_kernel(wkf, planner):
     assert "norm_rope ([2, 4, 5, 64] f32)" in dot and dot.count("->") >= 4
 
 
+@pytest.mark.parametrize("reference", [False, True])
+def test_a_product_with_written_out_weights_is_left_where_it_is_wanted(wkf, reference):
+    """Also where a copy of x has the product's shape: a square matrix, and x that starts behind its buffer's first element."""
+    dev = wkf.Device.planner()
+    if reference:
+        dev.set_fusion(wkf.FUSION_REFERENCE)
+    n, m = 6656, 1300
+    w = weights(wkf, dev, n, n, 128)
+    flat = zeros(wkf, dev, (m * n + 8,), F16)
+    for start in (0, 8):
+        x = flat.narrow(0, start, m * n).reshape([m, n]) if start else zeros(wkf, dev, (m, n), F16)
+        y = x.mat_mul_q4(w)
+        wkf.materialize_into([y], [wkf.Tensor.zeros(dev, (m, n), wkf.F16)])
+        kinds = [k.kind for k in y.kernels()]
+        assert kinds[-1] == "gemm" and kinds.count("q4_dense") == 1, kinds
+    dev.close()
+
+
 def test_extern_block_of_the_guide_matches_the_header():
     """The integration guide declares every function of wkf_decode.h with as many arguments."""
     text = re.sub(r"/\*.*?\*/", " ", open(os.path.join(ROOT, "include", "wkf_decode.h")).read(), flags=re.S)

@@ -243,10 +243,8 @@ TensorData Resolver::mat_mul_q4_dense(const Q4& w, const TensorData& x_in, const
   TensorData flat = out;
   flat.layout = Layout::contiguous({M, N});
   flat.layout.offset = out.layout.offset;
-  if (st_.fusion == FusionMode::Tree) mat_mul_out_ = &flat;
-  TensorData got = run_matmul(mm);
-  mat_mul_out_ = nullptr;
-  if (got.buffer.get() != flat.buffer.get()) copy_map(got, flat);
+  mat_mul_out_ = &flat;
+  run_matmul(mm);
   return out;
 }
 

@@ -232,7 +232,7 @@ TensorData Resolver::run_matmul(const NodeP& n) {
   } else {
     b = make_contiguous(b);
   }
-  if (M == 0 || N == 0 || batch == 0) return alloc(out_shape, a.dtype, false);
+  if (M == 0 || N == 0 || batch == 0) return alloc(out_shape, a.dtype, false, true);
   if (batch > 65535) throw Error(WKF_ERR_UNSUPPORTED, "mat_mul: more than 65535 matrices in a batch");
   if (M > 0xffffffffull || N > 0xffffffffull || K > 0xffffffffull) throw Error(WKF_ERR_UNSUPPORTED, "mat_mul: dimension does not fit 32 bits");
   auto slices_shape = [&](size_t slices) {  // partial sums: [slice][batch...][M][N]
@@ -270,7 +270,7 @@ TensorData Resolver::run_matmul(const NodeP& n) {
       // short walks of K cost more than the second launch)
       size_t chunk = (K + 7) / 8;
       chunk = (chunk + kblock - 1) / kblock * kblock;
-      TensorData out = alloc(out_shape, a.dtype, false);
+      TensorData out = alloc(out_shape, a.dtype, false, true);
       const std::string sig = std::string("gemm|gfx950|") + dtype_name(a.dtype) + "|skinny_bt|mfma32x32|block8";
       wkf_kernel* k = kernel(sig, [&] { return std::string("#define WKF_H ") + (a.dtype == DType::F16 ? "1" : "0") + "\n" + kGemmSkinnyBtBlock; });
       struct {
@@ -331,7 +331,7 @@ TensorData Resolver::run_matmul(const NodeP& n) {
       chunk = K;
     }
     TensorData part = whole_k ? TensorData() : alloc(slices_shape(S), DType::F32, false);
-    TensorData out_whole = whole_k ? alloc(out_shape, a.dtype, false) : TensorData();
+    TensorData out_whole = whole_k ? alloc(out_shape, a.dtype, false, true) : TensorData();
     size_t chunk_max = 256;
     while (chunk_max < chunk) chunk_max *= 2;
     if (whole_k) chunk_max = k_lds;
@@ -537,7 +537,7 @@ TensorData Resolver::run_matmul(const NodeP& n) {
       const size_t bm = 64 * size_t(ni), bn = 64 * size_t(nj);
       const size_t ftiles = ((M + bm - 1) / bm) * ((N + bn - 1) / bn);
       if (ftiles > 0x7fffffffull || S > 65535) throw Error(WKF_ERR_UNSUPPORTED, "mat_mul: too many tiles");
-      TensorData fout = sp ? alloc(slices_shape(S), DType::F32, false) : alloc(out_shape, a.dtype, false);
+      TensorData fout = sp ? alloc(slices_shape(S), DType::F32, false) : alloc(out_shape, a.dtype, false, true);
       std::string fsig = "gemm|gfx950|f16|mfma32x32x16|" + std::to_string(bm) + "x" + std::to_string(bn) + "x64|w2x2|direct to LDS|stages" + std::to_string(ns);
       if (sp) fsig += "|splitk";
       if (bt) fsig += "|bt";
@@ -619,7 +619,7 @@ TensorData Resolver::run_matmul(const NodeP& n) {
   const bool dma = dma_ok && !shortk && !stream;
   if (dma && !tail) nmain = tiles;
   const bool rotk = t128 && !split && N <= 128 && K >= 512 && K * N * dtype_size(a.dtype) <= (size_t(1) << 20);
-  TensorData out = split ? alloc(slices_shape(slices), DType::F32, false) : alloc(out_shape, a.dtype, false);
+  TensorData out = split ? alloc(slices_shape(slices), DType::F32, false) : alloc(out_shape, a.dtype, false, true);
   std::string sig = t128 ? std::string("gemm|gfx950|f16|mfma32x32x16|128x128x64|w2x2|edge") : gemm_signature(kind, a.dtype);
   // ragged f16 shapes (and K slices) on the large tile: buffer loads that read zeros past the edges, unless an offset
   // inside a tile could pass 32 bits or rows of C do not start 16-byte aligned; those keep 64-bit pointers

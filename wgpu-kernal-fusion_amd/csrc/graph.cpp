@@ -516,9 +516,10 @@ bool Resolver::try_map_table(const Program& prog, const std::vector<TensorData>&
 }
 
 TensorData Resolver::alloc(const std::vector<size_t>& shape, DType dt, bool zero, bool result) {
-  if (mat_mul_out_ && !zero && shape == mat_mul_out_->layout.shape && dt == mat_mul_out_->dtype) {
+  if (mat_mul_out_ && result) {
     const TensorData out = *mat_mul_out_;
     mat_mul_out_ = nullptr;
+    if (shape != out.layout.shape || dt != out.dtype) throw Error(WKF_ERR_UNSUPPORTED, "mat_mul: the product does not fit the output tensor");
     return out;
   }
   TensorData td;

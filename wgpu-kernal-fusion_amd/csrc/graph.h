@@ -202,7 +202,8 @@ class Resolver {
   // the table, or nothing when no value is worth it
   BufRef cut_table(Program& prog, const std::vector<TensorData>& in, size_t numel, std::string* what);
   void launch_map_tiled(MapSpec& spec, const Space& sp, const std::vector<TensorData>& in, const TensorData& out, bool in_place);
-  // `result`: the buffer receives the value of a reduce node (allocation-free mode: the caller's output tensor)
+  // `result`: the buffer receives the value of a reduce node (allocation-free mode: the caller's output tensor) or of a
+  // mat_mul node (mat_mul_out_)
   TensorData alloc(const std::vector<size_t>& shape, DType dt, bool zero, bool result = false);
   TensorData make_contiguous(const TensorData& td);
   void record(LaunchRecord&& r, wkf_kernel* k, const std::vector<unsigned char>& args);
@@ -213,8 +214,7 @@ class Resolver {
   bool team_launched_ = false;
   Settings st_;
   std::vector<LaunchRecord>* log_;
-  // where run_matmul leaves its product, taken by the one allocation of its shape and dtype (mat_mul_q4_dense sees to it
-  // that no temporary has both); null: a new buffer
+  // where run_matmul leaves its product: taken by the allocation of the product itself; null: a new buffer
   const TensorData* mat_mul_out_ = nullptr;
   std::set<const Node*> shared_;
   std::map<const Node*, TensorData> results_;       // roots whose kernels write the caller's output tensor
