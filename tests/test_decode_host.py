@@ -281,6 +281,18 @@ def test_a_product_with_written_out_weights_is_left_where_it_is_wanted(wkf, refe
     dev.close()
 
 
+def test_written_out_weights_are_f16_only(wkf, planner):
+    """Rows of f32 never take them, and the kernel's text has no variant for them."""
+    codes = np.zeros((64, 16 * 1024), np.uint8)
+    w = wkf.Q4Weights(planner, codes, np.ones((1, 16 * 1024), F16), group=64)
+    y, z = zeros(wkf, planner, (1100, 64), F16).mat_mul_q4(w), zeros(wkf, planner, (1100, 64), F32).mat_mul_q4(w)
+    y.materialize()
+    z.materialize()
+    written = [k for k in y.kernels() if k.kind == "q4_dense"]
+    assert len(written) == 1 and "WKF_H" not in wkf.kernel_source(written[0].signature)
+    assert not [k for k in z.kernels() if k.kind == "q4_dense"]
+
+
 def test_extern_block_of_the_guide_matches_the_header():
     """The integration guide declares every function of wkf_decode.h with as many arguments."""
     text = re.sub(r"/\*.*?\*/", " ", open(os.path.join(ROOT, "include", "wkf_decode.h")).read(), flags=re.S)

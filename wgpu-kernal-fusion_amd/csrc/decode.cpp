@@ -203,7 +203,7 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
 
 TensorData Resolver::mat_mul_q4_dense(const Q4& w, const TensorData& x_in, const TensorData& out, size_t M) {
   const size_t N = w.n, Kp = (w.k + 7) / 8 * 8;
-  const bool z = bool(w.zeros), h = x_in.dtype == DType::F16;
+  const bool z = bool(w.zeros);
   // rows of x that start on 16 bytes: what mat_mul would otherwise see to by itself
   TensorData x = x_in;
   x.layout.shape = {M, w.k};
@@ -215,8 +215,8 @@ TensorData Resolver::mat_mul_q4_dense(const Q4& w, const TensorData& x_in, const
     x = padded;
   }
   TensorData wt = alloc({N, Kp}, x.dtype, false);
-  const std::string sig = std::string("q4_dense|gfx950|") + dtype_name(x.dtype) + "|s" + dtype_name(w.scale_dtype) + (z ? "|zeros" : "");
-  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + define("WKF_H", h) + define("WKF_SH", w.scale_dtype == DType::F16) + define("WKF_Z", z) + kQ4Dense; });
+  const std::string sig = joined({"q4_dense|gfx950|s", dtype_name(w.scale_dtype), z ? "|zeros" : ""});
+  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + define("WKF_SH", w.scale_dtype == DType::F16) + define("WKF_Z", z) + kQ4Dense; });
   struct {
     const void *codes, *scales, *zeros;
     void* out;
