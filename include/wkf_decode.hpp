@@ -105,6 +105,22 @@ void materialize_into(const Tensor<R, D>& t, const Tensor<R, D>& out) {
   check(wkf_tensor_materialize_into(&from, 1, &to));
 }
 
+// One of several tensors and where it goes, in the braces of the call below; tensors of any rank and type stand beside each other.
+struct Into {
+  template <int R, class D>
+  Into(const Tensor<R, D>& t, const Tensor<R, D>& out) : from(t.handle()), to(out.handle()) {}
+  wkf_tensor *from, *to;
+};
+// materialize_into({{q, out_q}, {k, out_k}}): one pass over the joint graph, in which sibling norm_ropes are one launch.
+inline void materialize_into(std::initializer_list<Into> list) {
+  std::vector<wkf_tensor*> from, to;
+  for (const Into& i : list) {
+    from.push_back(i.from);
+    to.push_back(i.to);
+  }
+  check(wkf_tensor_materialize_into(from.data(), int(list.size()), to.data()));
+}
+
 }  // namespace wkf
 
 #endif

@@ -348,3 +348,42 @@ def test_the_typed_facade_compiles_and_plans(tmp_path):
     assert r.returncode == 0, r.stdout + r.stderr
     r = subprocess.run([str(tmp_path / "facade")], capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and r.stdout.strip() == "OK", r.stdout + r.stderr
+
+
+SIBLINGS = r"""
+    #include <cstdio>
+    #include <wkf_decode.hpp>
+    using namespace wkf;
+    int main() {
+      auto dev = Device::planner();
+      Tensor<1, F32> g(dev, {64}, std::vector<float>(64, 1.0f));
+      auto table = zeros<2, F32>(dev, {9, 32});
+      auto q = norm_rope(zeros<4, F16>(dev, {2, 4, 3, 64}), g, table, table, 1e-5f, {1, 6});
+      auto k = norm_rope(zeros<4, F16>(dev, {2, 2, 3, 64}), g, table, table, 1e-5f, {1, 6});
+      auto sum = Tensor<1, F32>(dev, {64}, std::vector<float>(64, 2.0f)) + g;
+      auto to_q = zeros<4, F16>(dev, {2, 4, 3, 64}), to_k = zeros<4, F16>(dev, {2, 2, 3, 64});
+      auto to_sum = zeros<1, F32>(dev, {64});
+      materialize_into({{q, to_q}, {k, to_k}});
+      const int together = wkf_tensor_kernel_count(q.handle());
+      materialize_into({{q, to_q}, {sum, to_sum}, {k, to_k}});
+      const int with_sum = wkf_tensor_kernel_count(q.handle());
+      int code = 0;
+      try { materialize_into({}); } catch (const Error& e) { code = e.code; }
+      std::printf("%d %d %d\n", together, with_sum, code);
+      return 0;
+    }
+"""
+
+
+def test_the_typed_facade_computes_siblings_together(tmp_path, wkf):
+    """q and k in one launch, tensors of other ranks and types beside them."""
+    gxx, libdir = shutil.which("g++"), os.path.join(ROOT, "wgpu-kernal-fusion_amd")
+    if gxx is None:
+        pytest.skip("no g++ on this machine")
+    (tmp_path / "siblings.cpp").write_text(SIBLINGS)
+    r = subprocess.run([gxx, "-std=c++17", "-O1", "-Wall", "-Wextra", "-Werror", "-I", os.path.join(ROOT, "include"), str(tmp_path / "siblings.cpp"), "-o", str(tmp_path / "siblings"),
+                        "-L", libdir, "-lwkf_hip", f"-Wl,-rpath,{libdir}"], capture_output=True, text=True)
+    assert r.returncode == 0, r.stdout + r.stderr
+    r = subprocess.run([str(tmp_path / "siblings")], capture_output=True, text=True, timeout=300)
+    counts = r.stdout.split()
+    assert r.returncode == 0 and counts[0] == "1" and int(counts[1]) in (2, 3) and counts[2] == str(wkf.ERR_INVALID_ARG), r.stdout + r.stderr
