@@ -674,6 +674,75 @@ def test_attend_gives_the_same_bits_every_time(gpu):
             assert np.array_equal(computed(t), first)
 
 
+# ---- attention of sequences with different numbers of rows -----------------------------------------------------------
+
+def check_attend_by(kernel, gpu, dtype, lengths, counts, heads, kv, dim, block, rows=None, causal=True, scale=None, seed=0):
+    """As check_attend, by a kernel of this name; rows of q behind a count are NaN, and their results zeros."""
+    rows = max(counts) if rows is None else rows
+    rng = rng_of(60, seed, dim, block, rows, *lengths)
+    cache, held, _ = filled(gpu, rng, dtype, lengths, kv, dim, block)
+    q = rng.standard_normal((len(lengths), heads, rows, dim)).astype(dtype)
+    for b, n in enumerate(counts):
+        q[b, :, n:] = np.nan
+    scale = np.float32(dim ** -0.5 if scale is None else scale).astype(np.float64)
+    t = leaf(gpu, q).attend(cache, scale, causal, counts)
+    t.materialize()
+    assert [i.kind for i in t.kernels()] == [kernel], [(i.kind, i.detail) for i in t.kernels()]
+    got = computed(t)
+    for b, n in enumerate(lengths):
+        case = (q[b, :, :counts[b]], *held[b], scale, causal, n, counts[b])
+        want, slack = ref.attend(*case)
+        if dtype == F16:
+            slack = slack + ref.f16_weights_slack(*case)
+        ref.close(got[b, :, :counts[b]], want, dtype, slack, f"sequence {b}")
+        assert np.all(got[b, :, counts[b]:] == 0), f"sequence {b}"
+    return t, got
+
+
+MIXED_CASES = [  # lengths, counts, heads, kv heads, dim, block, rows
+    ([3000, 2500, 40, 700], [200, 1, 1, 3], 8, 2, 64, 32, 200), ([5000, 131, 64, 5000], [1, 130, 0, 1], 16, 4, 128, 64, 131),
+    ([4000, 3900, 4000], [0, 2, 0], 4, 2, 80, 128, 33), ([4000, 3000, 100], [1, 0, 0], 4, 1, 20, 32, 9), ([0, 3000, 0, 2000], [0, 17, 0, 16], 2, 2, 256, 64, 18),
+    ([900] * 9 + [6000], [1] * 9 + [50], 6, 3, 96, 64, 50), ([2000, 1], [5, 1], 12, 2, 64, 32, 100),
+]
+
+
+@DTYPES
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("case", MIXED_CASES, ids=str)
+def test_attend_of_a_chunk_beside_single_tokens(gpu, case, causal, dtype):
+    lengths, counts, heads, kv, dim, block, rows = case
+    t, got = check_attend_by("attend_rows", gpu, dtype, lengths, counts, heads, kv, dim, block, rows, causal)
+    for _ in range(3):
+        assert np.array_equal(computed(t), got)
+
+
+# so many rows of like sequences that tiles of 128 fill the chip
+FULL_CASES = [([150, 0, 129, 200], [129, 0, 129, 129], 96, 96, 64, 64), ([100, 37, 300, 1, 128, 0], [100, 37, 100, 1, 100, 0], 150, 50, 72, 32),
+              ([141, 140, 0, 270, 64, 33], [140, 140, 0, 140, 64, 33], 96, 48, 128, 128), ([260] * 4, [256] * 4, 32, 32, 128, 64), ([400, 260], [200, 200], 128, 64, 16, 32)]
+
+
+@DTYPES
+@pytest.mark.parametrize("case", FULL_CASES, ids=str)
+def test_attend_with_full_tiles(gpu, case, dtype):
+    check_attend_by("attend_prompt", gpu, dtype, *case)
+
+
+@pytest.mark.parametrize("dtype,lengths,counts,heads,kv,dim,block", [(F32, [70, 66, 0, 5, 65, 64, 71, 74], [70, 66, 0, 5, 65, 64, 70, 70], 96, 48, 200, 32), (F32, [70, 66, 0, 70], [70, 66, 0, 70], 160, 80, 255, 32),
+                                                                     (F32, [300, 280], [140, 140], 112, 56, 130, 64), (F16, [300, 280], [140, 140], 112, 56, 130, 64),
+                                                                     (F16, [128, 128, 127, 128], [128, 128, 0, 127], 344, 86, 200, 32)], ids=str)
+def test_attend_with_full_tiles_of_large_heads(gpu, dtype, lengths, counts, heads, kv, dim, block):
+    check_attend_by("attend_prompt", gpu, dtype, lengths, counts, heads, kv, dim, block)
+
+
+@DTYPES
+def test_attend_with_full_tiles_in_other_ways(gpu, dtype):
+    check_attend_by("attend_prompt", gpu, dtype, [150, 0, 190, 65], [70, 0, 70, 65], 192, 192, 64, 32, causal=False)
+    check_attend_by("attend_prompt", gpu, dtype, [150, 0, 190, 65], [70, 0, 70, 33], 192, 192, 64, 32)
+    check_attend_by("attend_prompt", gpu, dtype, [150, 0, 190, 65], [64, 0, 100, 65], 192, 96, 64, 64, causal=False)
+    for scale in (0.0, 4.0):
+        check_attend_by("attend_prompt", gpu, dtype, [150, 10, 190, 65], [70, 10, 70, 65], 192, 192, 64, 64, scale=scale)
+
+
 # ---- together ---------------------------------------------------------------------------------------------------
 
 @DTYPES

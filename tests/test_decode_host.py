@@ -293,6 +293,26 @@ def test_written_out_weights_are_f16_only(wkf, planner):
     assert not [k for k in z.kernels() if k.kind == "q4_dense"]
 
 
+def test_rows_behind_a_count_are_no_work(wkf, planner):
+    """A chunk of a prompt beside single tokens over long caches: the kernel that splits the caches, and as many workgroups
+    for that as for the same rows without the empty ones."""
+    cache = wkf.KvCache(planner, 4, 8, 64, 8192, 64)
+    k = zeros(wkf, planner, (4, 8, 8192, 64), F16)
+    cache.append(k, k)
+
+    def launched(rows, counts):
+        t = zeros(wkf, planner, (4, 32, rows, 64), F16).attend(cache, counts=counts)
+        t.materialize()
+        (launch,) = t.kernels()
+        return launch.kind, dict(p.split("=") for p in launch.detail.split())
+
+    kind, mixed = launched(256, [256, 1, 1, 1])
+    assert kind == "attend_rows" and 512 <= int(mixed["workgroups"]) <= 640
+    alone, behind = launched(2, [2, 1, 0, 1]), launched(15, [2, 1, 0, 1])
+    assert alone[0] == behind[0] == "attend_rows" and alone[1]["workgroups"] == behind[1]["workgroups"]
+    assert launched(1024, [1024] * 4)[0] == "attend_prompt"
+
+
 def test_extern_block_of_the_guide_matches_the_header():
     """The integration guide declares every function of wkf_decode.h with as many arguments."""
     text = re.sub(r"/\*.*?\*/", " ", open(os.path.join(ROOT, "include", "wkf_decode.h")).read(), flags=re.S)

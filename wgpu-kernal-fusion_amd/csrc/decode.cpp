@@ -425,7 +425,7 @@ struct AttendArgs {
   uint64_t sb, sh, ss;
   uint32_t heads, share, rows, seqs, cap, causal;
   float scale;
-  uint32_t span, tiles, pad;
+  uint32_t span, tiles, walks;
   uint32_t len[NB], cnt[NB], start[NB];
 };
 template <size_t NB>
@@ -542,11 +542,28 @@ TensorData Resolver::run_attend(const NodeP& n) {
   const size_t R = n->shape.size(), rows = n->shape[R - 2], heads = n->shape[R - 3];
   if (!out.layout.numel()) return out;
   const size_t nb = room_for(c.seqs), share = heads / c.heads, tiles = (share * rows + 15) / 16;
-  // Rows enough to give every compute unit a tile of 128: the kernel that spreads the codes in the LDS for all of them
-  // (2048 new tokens after 2048, 32/8 heads: 512 tiles, 121 us against 276 in tiles of 16 rows).  With fewer tiles the cache has
-  // to be split over workgroups, which the kernel for tiles of 16 rows does (512 new tokens after 3584: 101 us against 89).
+  wkf_props props;
+  if (wkf_device_props(dev_, &props) != WKF_OK) throw Error(WKF_ERR_HIP, wkf_last_error());
+  const size_t cus = size_t(std::max(1, props.compute_units));
+  // Many rows take the kernel that spreads the codes in the LDS for 128 of them; it does not split a cache over workgroups, which
+  // the kernel for tiles of 16 rows does.  What counts is how many full tiles of the longest sequence's length all rows come
+  // to, each by its own sequence: rows behind a count are no work, and one token over a long cache is one row of a tile that
+  // walks all of it alone (2048 new tokens beside 15 single ones over 32768, 32/8 heads of 128 in f16: 35 such tiles, 431 us
+  // in tiles of 16 rows and 1408 in tiles of 128; beside 15 over 2000: 516, 285 and 228).  The two meet at about 145 of them in f16
+  // (new tokens after 3500, 32/8 heads of 128: 512, which are 128, 89 and 101; 768 after 3072, 192, 132 and 113), at 190 where a tile
+  // takes a compute unit alone (f32, heads of 128: 768 tokens 262 and 261, 1024 tokens 350 and 277), and at a thousand where the
+  // registers do not hold its sums (f16, heads of 256: 2048 after 2048, 512 of them, 541 and 591; four prompts of 2048: 995 and 889).
+  double work = 0;
+  size_t furthest = 0;
+  for (size_t b = 0; b < c.seqs; b++) {
+    if (!args.counts[b]) continue;
+    work += double(c.heads * share * args.counts[b]) * c.len[b];
+    furthest = std::max<size_t>(furthest, c.len[b]);
+  }
+  const bool h = n->dtype == DType::F16;
+  const double full = double(cus) * (!h ? 0.75 : c.dp <= 128 ? 0.5625 : c.dp <= 192 ? 0.75 : 4.0);
   const size_t big = (share * rows + 127) / 128;
-  if (share * rows > 64 && big * c.heads * c.seqs >= 256) {
+  if (share * rows > 64 && furthest && work >= full * 128 * double(furthest)) {
     const std::string psig = kv_signature("attend_prompt", c, n->dtype, nb);
     wkf_kernel* pk = kernel(psig, [&] { return std::string(kPrelude) + kv_defines(c, n->dtype, nb) + kKvLayout + kKvCodes + kAttendPrompt; });
     with_room<PromptArgs>(nb, [&](auto& a) {
@@ -573,50 +590,59 @@ TensorData Resolver::run_attend(const NodeP& n) {
     return out;
   }
   // How many groups of 32 tokens a workgroup takes: so few that there are nearly as many workgroups as the chip holds at once
-  // (512; large heads leave registers for 256), and no more, where a second round would begin (16 sequences of 17000 to 32768
+  // (two a compute unit; large heads leave registers for one), and no more, where a second round would begin (16 sequences of 17000 to 32768
   // tokens, 8 key heads: 149 us, against 174 with 304 workgroups; 8 sequences of up to 3000, 8 heads of 256: 26 us, 33 with
   // 512).  Joining s parts costs about as much as reading s groups, so a few long sequences are split no finer than the square
   // root of twice their groups (one sequence, 8 key heads: 4000 tokens 16.6 us in 32 parts, 11.9 in 8; 16000 tokens 21.4 us in 32
   // parts, 19.3 in 16).  Up to 16 groups stay whole: the join alone takes 3 us.
-  size_t total = 0, longest = 0;
-  for (uint32_t n : c.len) {
-    total += (n + 31) / 32;
-    longest = std::max<size_t>(longest, (n + 31) / 32);
+  // Rows behind a sequence's count see nothing: only the tiles up to it are work.
+  size_t total = 0, longest = 0, units = 0;
+  std::vector<size_t> live(c.seqs), groups(c.seqs);  // tiles of a key head with rows that see tokens, groups that its rows walk
+  for (size_t b = 0; b < c.seqs; b++) {
+    live[b] = (share * args.counts[b] + 15) / 16;
+    groups[b] = live[b] ? (c.len[b] + 31) / 32 : 0;
+    total += c.heads * live[b] * groups[b];
+    units += c.heads * live[b];
+    longest = std::max(longest, groups[b]);
   }
   constexpr size_t waves = 4, ahead = 2;
-  const size_t each = c.heads * tiles, resident = c.dp <= 128 ? 512 : 256;
-  size_t span = longest <= 16 ? longest : std::max((total * each + resident - 1) / resident, size_t(std::ceil(std::sqrt(2.0 * double(longest)))));
+  const size_t resident = c.dp <= 128 ? 2 * cus : cus;
+  size_t span = longest <= 16 ? longest : std::max((total + resident - 1) / resident, size_t(std::ceil(std::sqrt(2.0 * double(longest)))));
   span = std::max(waves, (span + waves - 1) / waves * waves);
   // Sequences and heads that are more than that by themselves stay whole (64 of 2000 to 4000 tokens, 8 heads: 81 us, 88 in
   // parts), unless some are much longer than the average: half as many again are for those (one of 32000 tokens among 63 of
   // 300: 32 us against 194).  Many times as many keep the chip busy in any case, and their parts would take too much memory.
-  const size_t units = c.seqs * each, most = std::max(resident, units + (longest > 2 * total / c.seqs ? resident / 2 : 0));
+  const size_t most = std::max(resident, units + (longest * units > 2 * total ? resident / 2 : 0));
   if (units > 32 * resident) span = std::max(span, (longest + waves - 1) / waves * waves);
+  auto parts = [&](size_t b) { return std::max<size_t>(1, (groups[b] + span - 1) / span); };
   while (span < longest) {
     size_t workgroups = 0;
-    for (uint32_t n : c.len) workgroups += each * std::max<size_t>(1, ((n + 31) / 32 + span - 1) / span);
+    for (size_t b = 0; b < c.seqs; b++) workgroups += c.heads * live[b] * parts(b);
     if (workgroups <= most) break;
     span += (span / 16 + waves) / waves * waves;
   }
-  std::vector<uint32_t> start;  // the splits of the sequences before each
-  size_t splits = 0;
-  for (uint32_t n : c.len) {
-    start.push_back(uint32_t(splits));
-    splits += std::max<size_t>(1, ((n + 31) / 32 + span - 1) / span);
+  std::vector<uint32_t> start;  // the workgroups of the sequences before each
+  size_t walks = 0, dead = 0;
+  bool split = false;
+  for (size_t b = 0; b < c.seqs; b++) {
+    start.push_back(uint32_t(walks));
+    walks += c.heads * live[b] * parts(b);
+    split |= parts(b) > 1;
+    if (live[b] < tiles) dead = c.seqs * c.heads * tiles;
   }
-  const bool split = splits > c.seqs;
+  const uint32_t grid = grid_dim(walks + dead, "attend");
   TensorData part, stat;
   if (split) {
-    part = alloc({splits, each, 16, c.dp}, DType::F32, false);
-    stat = alloc({splits, each, 32}, DType::F32, false);
-    if (units > c.counters) {  // zeros, and every launch leaves zeros
-      c.done = alloc({units}, DType::F32, true).buffer;
-      c.counters = units;
+    part = alloc({walks, 16, c.dp}, DType::F32, false);
+    stat = alloc({walks, 32}, DType::F32, false);
+    if (walks > c.counters) {  // zeros, and every launch leaves zeros
+      c.done = alloc({walks}, DType::F32, true).buffer;
+      c.counters = walks;
     }
   }
   const std::string sig = kv_signature("attend_rows", c, n->dtype, nb) + "|w" + std::to_string(waves);
   wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + define("W", waves) + define("AHEAD", ahead) + kv_defines(c, n->dtype, nb) + kKvLayout + kKvCodes + kAttendRows; });
-  const std::string d = detail({{"sequences", c.seqs}, {"heads", heads}, {"kv_heads", c.heads}, {"rows", rows}, {"dim", c.dim}, {"splits", splits}});
+  const std::string d = detail({{"sequences", c.seqs}, {"heads", heads}, {"kv_heads", c.heads}, {"rows", rows}, {"dim", c.dim}, {"workgroups", walks}});
   with_room<AttendArgs>(nb, [&](auto& a) {
     const Strides4 st(q.layout);
     a.q = first(q);
@@ -638,10 +664,11 @@ TensorData Resolver::run_attend(const NodeP& n) {
     a.scale = args.scale;
     a.span = uint32_t(span);
     a.tiles = uint32_t(tiles);
+    a.walks = uint32_t(walks);
     std::copy(c.len.begin(), c.len.end(), a.len);
     std::copy(args.counts.begin(), args.counts.end(), a.cnt);
     std::copy(start.begin(), start.end(), a.start);
-    launch("attend_rows", sig, d, k, grid_dim(splits * each, "attend"), 1, 1, uint32_t(64 * waves), a);
+    launch("attend_rows", sig, d, k, grid, 1, 1, uint32_t(64 * waves), a);
   });
   return out;
 }

@@ -40,7 +40,7 @@ struct KvCache {
   size_t seqs = 0, heads = 0, dim = 0, dp = 0, block = 0;
   size_t capacity = 0, cap = 0;  // tokens of a sequence: what was asked for, and rounded up to whole blocks and to 64
   BufRef codes, scales, staged;
-  BufRef done;          // split attention: parts finished, a counter for each sequence, head and tile of rows
+  BufRef done;          // split attention: parts finished, a counter for each workgroup
   size_t counters = 0;
   std::mutex mu;  // lengths, slots and generation; held while a launch that goes by them is put on the stream
   std::vector<uint32_t> len;
