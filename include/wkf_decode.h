@@ -12,7 +12,8 @@
  * wkf_tensor_materialize_into computes lazy tensors into such tensors, wkf_tensor_device_ptr says where one lies.
  *
  * Element types are those of the Tensor API (WKF_F32, WKF_F16); sums, softmax statistics and norms are kept in f32 and
- * results are rounded once.  Every size below is in elements.
+ * results are rounded once.  On the way to f16 results a product with many rows may round weights to f16 too, an error like
+ * the result's own; after wkf_device_set_exact_math(dev, 1) none does.  Every size below is in elements.
  */
 #ifndef WKF_DECODE_H
 #define WKF_DECODE_H
@@ -52,7 +53,7 @@ int wkf_q4_new(wkf_device* dev, size_t k, size_t n, size_t group, const void* co
 void wkf_q4_free(wkf_q4* w);
 int wkf_q4_shape(const wkf_q4* w, size_t* k, size_t* n, size_t* group);
 /* x [..., M, k] times W [k, n]: [..., M, n] in x's dtype, with at most 2^20 - 1 rows of x in all.  With many rows of f16 each
- * weight may be rounded to f16 first, if none of them is too large or too small for its normal numbers. */
+ * weight may be rounded to f16 first, if none of them is too large or too small for its normal numbers (never with exact math). */
 int wkf_tensor_mat_mul_q4(const wkf_tensor* x, const wkf_q4* w, wkf_tensor** out);
 
 /* ---- the norm of a head and its rotation ---- */
@@ -93,6 +94,7 @@ int wkf_kv_cache_values(wkf_kv_cache* c, int dtype, size_t first, size_t count, 
  * softmax(scale q k^T) v.  Head h reads key head h / (heads / kv_heads).  The S rows are the LAST tokens of each sequence, or
  * its last counts[b] <= S ones (then rows behind counts[b] give zeros); with causal != 0 a row sees the tokens up to its own,
  * else all of its sequence.  A row that sees no token gives zeros.  scale is finite and not negative.
+ * With more than 16 rows of f16 for a key head its softmax weights may be rounded to f16 (never with exact math).
  * The node stands for the cache as it is now: materialising it after an append or a reset is WKF_ERR_INVALID_ARG. */
 int wkf_tensor_attend(const wkf_tensor* q, wkf_kv_cache* c, float scale, int causal, const size_t* counts, wkf_tensor** out);
 

@@ -70,7 +70,8 @@ int wkf_device_get_fusion(wkf_device* dev);
  *   evaluated in f64 and rounded once (it equals the correctly rounded f32 value,
  *   so later ops cannot amplify an error); the last op before a store uses the
  *   f32 library (<= 1-2 ulp); values that only feed a reduction use the f32 library.
- * exact != 0: every transcendental op is evaluated in f64 and rounded once. */
+ * exact != 0: every transcendental op is evaluated in f64 and rounded once, and the operators of wkf_decode.h round no
+ *   weight of a softmax or of a matrix to f16 on the way to an f16 result. */
 int wkf_device_set_exact_math(wkf_device* dev, int exact);
 
 /* Rows longer than one workgroup's registers (no reference counterpart: the reference's reduce takes a row of any

@@ -133,3 +133,10 @@ def f16_weights_slack(q, k, v, scale, causal, length, count):
     f16 subnormals is 2^-24, half of it 2^-25) times the largest value, for each token."""
     a, _ = attend(q, k, np.abs(v), scale, causal, length, count)
     return U16 * a + length * 2.0 ** -37 * (np.abs(v).max() if v.size else 0.0)
+
+
+def two_part_weights_slack(q, k, v, scale, causal, length, count):
+    """What softmax weights in two parts of f16 may add.  The first part is off by half a step, which f32 holds exactly; the second
+    is that, off by half a step of its own: U16^2 = 4 U32 of the weight.  Below f16's normal numbers: as in f16_weights_slack."""
+    a, _ = attend(q, k, np.abs(v), scale, causal, length, count)
+    return U16 * U16 * a + length * 2.0 ** -37 * (np.abs(v).max() if v.size else 0.0)

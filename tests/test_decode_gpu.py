@@ -743,6 +743,77 @@ def test_attend_with_full_tiles_in_other_ways(gpu, dtype):
         check_attend_by("attend_prompt", gpu, dtype, [150, 10, 190, 65], [70, 10, 70, 65], 192, 192, 64, 64, scale=scale)
 
 
+# ---- without roundings to f16 on the way -----------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("kernel,lengths,counts,heads,kv,dim,block,exact", [
+    ("attend_rows", [1000, 0, 33], [1, 0, 1], 32, 8, 128, 64, False), ("attend_rows", [3000], [3], 5, 1, 64, 32, False), ("attend_rows", [700, 130], [2, 2], 16, 2, 256, 128, False),
+    ("attend_rows", [300, 4000], [40, 1], 4, 2, 80, 32, True), ("attend_rows", [333], [50], 40, 1, 20, 64, True),
+    ("attend_prompt", [150, 0, 129, 200], [129, 0, 129, 129], 96, 96, 64, 64, True), ("attend_prompt", [260] * 4, [256] * 4, 32, 32, 128, 64, True),
+    ("attend_prompt", [128, 128, 127, 128], [128, 128, 0, 127], 344, 86, 200, 32, True)], ids=str)
+def test_attend_in_f16_with_weights_of_22_bits(gpu, kernel, lengths, counts, heads, kv, dim, block, exact):
+    """One tile of rows a key head, and any number of them under exact math."""
+    rng = rng_of(62, dim, *lengths)
+    cache, held, _ = filled(gpu, rng, F16, lengths, kv, dim, block)
+    q = rng.standard_normal((len(lengths), heads, max(counts), dim)).astype(F16)
+    scale = np.float32(dim ** -0.5).astype(np.float64)
+    t = leaf(gpu, q).attend(cache, scale, True, counts)
+    gpu.set_exact_math(exact)
+    try:
+        t.materialize()
+        assert [i.kind for i in t.kernels()] == [kernel]
+        got = computed(t)
+    finally:
+        gpu.set_exact_math(False)
+    for b, n in enumerate(lengths):
+        case = (q[b], *held[b], scale, True, n, counts[b])
+        want, slack = ref.attend(*case)
+        ref.close(got[b], want, F16, slack + ref.two_part_weights_slack(*case), f"sequence {b}")
+
+
+@pytest.mark.parametrize("lengths,rows,exact", [([1000], 1, False), ([3000, 700], 2, False), ([700, 650], 60, True)], ids=str)
+def test_attend_in_f16_errs_by_the_rounding_of_its_result(gpu, lengths, rows, exact):
+    """In the 2-norm.  A rounding is spread evenly over half a step to both sides: its square is step^2 / 12 on average.  The
+    step is 2^-10 of the power of two below the value, and the square of that power over the value's is on average (1 - 1/4) /
+    (2 ln 2) where significands are spread as 1 / m: 2.07e-4 of the result.  Ten thousand values come within 1 % of that, 10 % are
+    allowed; one more rounding of each weight makes it 2.6e-4 and more."""
+    w, rng = load_package(), rng_of(64, rows, *lengths)
+    cache, held, _ = filled(gpu, rng, F16, lengths, 8, 128, 64, spread=False)
+    q = rng.standard_normal((len(lengths), 32, rows, 128)).astype(F16)
+    gpu.set_exact_math(exact)
+    try:
+        got = computed(leaf(gpu, q).attend(cache)).astype(np.float64)
+    finally:
+        gpu.set_exact_math(False)
+    scale = np.float32(128 ** -0.5).astype(np.float64)
+    want = np.stack([ref.attend(q[b], *held[b], scale, True, n, rows)[0] for b, n in enumerate(lengths)])
+    normal = np.abs(want) >= 2.0 ** -14
+    off = np.sqrt(np.square(got - want)[normal].sum() / np.square(want)[normal].sum())
+    assert off < 1.1 * 2.0 ** -10 * np.sqrt(0.75 / (2 * np.log(2)) / 12), off
+
+
+Q4_MANY = [(1100, 130, 7700, 128, True, F16), (800, 72, 11001, 32, False, F32), (1100, 130, 2000, 128, True, F16), (768, 64, 64, 32, False, F16), (800, 264, 300, 96, True, F32)]
+
+
+@pytest.mark.parametrize("exact", [False, True])
+@pytest.mark.parametrize("case", Q4_MANY, ids=lambda c: "x".join(str(v) for v in c[:4]))
+def test_mat_mul_q4_rounds_weights_only_where_it_writes_them_out(gpu, case, exact):
+    w, (m, k, n, group, zeros, sdt) = load_package(), case
+    rng = rng_of(63, m, k, n, group)
+    codes, scales, z = ref.q4_weights(rng, k, n, group, zeros, sdt)
+    x = rng.standard_normal((m, k)).astype(F16)
+    y = leaf(gpu, x).mat_mul_q4(w.Q4Weights(gpu, codes, scales, z, group))
+    gpu.set_exact_math(exact)
+    try:
+        y.materialize()
+        written = "q4_dense" in [i.kind for i in y.kernels()]
+        got = computed(y)
+    finally:
+        gpu.set_exact_math(False)
+    assert written == (n > 7000 and not exact)
+    dense = ref.q4_dense(codes, scales, z, group)
+    ref.close(got, x.astype(np.float64) @ dense, F16, ref.q4_slack(x, dense, written), str(case))
+
+
 # ---- together ---------------------------------------------------------------------------------------------------
 
 @DTYPES

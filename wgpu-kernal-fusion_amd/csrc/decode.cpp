@@ -133,8 +133,8 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
   // Many f16 rows: where no tiles below cover the product with one round of the chip, the weights are written out once, each
   // rounded to f16, and the product is mat_mul's ([1024,4096]x[4096,11008]: 114 us against 122 in tiles of 4-bit weights;
   // [1024,11008]x[11008,4096], which one round covers: 154 against 104).  Weights that would overflow or lose bits in f16
-  // stay in the tiles, which round none.
-  if (h && w.fits_f16 && M >= 768 && tiles_of(4, 32) > 256 && w.tiles_n() <= 65535) return mat_mul_q4_dense(w, x, out, M);
+  // stay in the tiles, which round none, and so does everything where the caller wants exact math ([1024,4096]x[4096,11008]: 128).
+  if (h && w.fits_f16 && !st_.exact_math && M >= 768 && tiles_of(4, 32) > 256 && w.tiles_n() <= 65535) return mat_mul_q4_dense(w, x, out, M);
   // the k = 32 steps of a tile that surely share a group, and the group in units of so many
   const size_t step = w.group % 128 == 0 ? 4 : w.group % 64 == 0 ? 2 : 1, units = w.group / (32 * step);
   int shift = -1;
@@ -564,8 +564,9 @@ TensorData Resolver::run_attend(const NodeP& n) {
   const double full = double(cus) * (!h ? 0.75 : c.dp <= 128 ? 0.5625 : c.dp <= 192 ? 0.75 : 4.0);
   const size_t big = (share * rows + 127) / 128;
   if (share * rows > 64 && furthest && work >= full * 128 * double(furthest)) {
-    const std::string psig = kv_signature("attend_prompt", c, n->dtype, nb);
-    wkf_kernel* pk = kernel(psig, [&] { return std::string(kPrelude) + kv_defines(c, n->dtype, nb) + kKvLayout + kKvCodes + kAttendPrompt; });
+    const size_t weight_parts = !h ? 3 : st_.exact_math ? 2 : 1;
+    const std::string psig = kv_signature("attend_prompt", c, n->dtype, nb) + joined({"|p", weight_parts});
+    wkf_kernel* pk = kernel(psig, [&] { return std::string(kPrelude) + define("WEIGHT_PARTS", weight_parts) + kv_defines(c, n->dtype, nb) + kKvLayout + kKvCodes + kAttendPrompt; });
     with_room<PromptArgs>(nb, [&](auto& a) {
       const Strides4 st(q.layout);
       a.q = first(q);
@@ -640,8 +641,12 @@ TensorData Resolver::run_attend(const NodeP& n) {
       c.counters = walks;
     }
   }
-  const std::string sig = kv_signature("attend_rows", c, n->dtype, nb) + "|w" + std::to_string(waves);
-  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + define("W", waves) + define("AHEAD", ahead) + kv_defines(c, n->dtype, nb) + kKvLayout + kKvCodes + kAttendRows; });
+  // A second part of f16 weights costs next to nothing where memory or latency bounds the kernel, with one tile of rows
+  // (one token over 1000: 9.2 us and 9.4; 16 sequences of up to 32768: 148 and 149), and more where the products do (512 new
+  // tokens after 3584: 87 and 98 us; in tiles of 128, 2048 after 2048: 126 and 169): there it is the caller's choice.
+  const size_t weight_parts = !h ? 3 : st_.exact_math || tiles == 1 ? 2 : 1;
+  const std::string sig = kv_signature("attend_rows", c, n->dtype, nb) + joined({"|w", waves, "|p", weight_parts});
+  wkf_kernel* k = kernel(sig, [&] { return std::string(kPrelude) + define("W", waves) + define("WEIGHT_PARTS", weight_parts) + define("AHEAD", ahead) + kv_defines(c, n->dtype, nb) + kKvLayout + kKvCodes + kAttendRows; });
   const std::string d = detail({{"sequences", c.seqs}, {"heads", heads}, {"kv_heads", c.heads}, {"rows", rows}, {"dim", c.dim}, {"workgroups", walks}});
   with_room<AttendArgs>(nb, [&](auto& a) {
     const Strides4 st(q.layout);
