@@ -89,6 +89,12 @@ uint32_t grid_dim(size_t v, const char* what, size_t threads = 256) {
   return uint32_t(v);
 }
 
+size_t compute_units(wkf_device* dev) {
+  wkf_props props;
+  if (wkf_device_props(dev, &props) != WKF_OK) throw Error(WKF_ERR_HIP, wkf_last_error());
+  return size_t(std::max(1, props.compute_units));
+}
+
 std::string kv_defines(const KvCache& c, DType dt, size_t nb) {
   return define("WKF_H", dt == DType::F16) + define("D", c.dim) + define("DP", c.dp) + define("T", c.block) + define("NB", nb);
 }
@@ -129,12 +135,13 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
   if (!M) return out;
   if (M > 0xfffffull) throw Error(WKF_ERR_UNSUPPORTED, "mat_mul_q4: more than 2^20 - 1 rows");
   const bool z = bool(w.zeros), h = x.dtype == DType::F16;
+  const size_t cus = compute_units(dev_);
   auto tiles_of = [&](size_t mt, size_t columns) { return (M + 16 * mt - 1) / (16 * mt) * ((w.tiles_n() + columns - 1) / columns); };
   // Many f16 rows: where no tiles below cover the product with one round of the chip, the weights are written out once, each
   // rounded to f16, and the product is mat_mul's ([1024,4096]x[4096,11008]: 114 us against 122 in tiles of 4-bit weights;
   // [1024,11008]x[11008,4096], which one round covers: 154 against 104).  Weights that would overflow or lose bits in f16
   // stay in the tiles, which round none, and so does everything where the caller wants exact math ([1024,4096]x[4096,11008]: 128).
-  if (h && w.fits_f16 && !st_.exact_math && M >= 768 && tiles_of(4, 32) > 256 && w.tiles_n() <= 65535) return mat_mul_q4_dense(w, x, out, M);
+  if (h && w.fits_f16 && !st_.exact_math && M >= 768 && tiles_of(4, 32) > cus && w.tiles_n() <= 65535) return mat_mul_q4_dense(w, x, out, M);
   // the k = 32 steps of a tile that surely share a group, and the group in units of so many
   const size_t step = w.group % 128 == 0 ? 4 : w.group % 64 == 0 ? 2 : 1, units = w.group / (32 * step);
   int shift = -1;
@@ -144,7 +151,7 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
   auto defines = [&] { return define("WKF_H", h) + define("WKF_SH", w.scale_dtype == DType::F16) + define("WKF_Z", z) + define("STEP", step) + define("POW2", shift >= 0); };
   const std::string d = detail({{"m", M}, {"n", N}, {"k", w.k}, {"group", w.group}});
   // More than 16 rows share x in the LDS; up to 32 beside few columns do not pay for it (24 rows of [4096,4096]: 9.5 us against 12.4).
-  if (M > (w.tiles_n() <= 256 ? 32 : 16)) {
+  if (M > (w.tiles_n() <= cus ? 32 : 16)) {
     // The smallest tiles of which the chip takes all at once, one a compute unit: larger ones read x less often, smaller ones
     // have K shared by more groups of waves ([4096,4096] f16: 256 rows 19.7 us in 32 x 128, 28.7 in 32 x 64, 28.3 in 64 x 128;
     // 1024 rows 42 in 64 x 256, 54 in 64 x 128; f32 256 rows 46 in 32 x 128, 70 in 32 x 64, 67 in 32 x 256).
@@ -153,7 +160,7 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
     };
     static constexpr Tile f16_tiles[] = {{2, 1, 4, 4}, {2, 2, 4, 4}, {4, 2, 4, 2}, {4, 2, 8, 1}, {4, 4, 8, 1}}, f32_tiles[] = {{2, 1, 4, 2}, {2, 1, 8, 2}, {2, 2, 8, 1}};
     const Tile *tile = h ? f16_tiles : f32_tiles, *last = h ? std::end(f16_tiles) - 1 : std::end(f32_tiles) - 1;
-    while (tile < last && tiles_of(tile->mt, tile->nt * tile->nw) > 256) tile++;
+    while (tile < last && tiles_of(tile->mt, tile->nt * tile->nw) > cus) tile++;
     const size_t mt = tile->mt, nt = tile->nt, nw = tile->nw, kw = tile->kw;
     constexpr size_t depth = 2;
     const void* rows = first(x);
@@ -436,7 +443,7 @@ struct PromptArgs {
   uint64_t sb, sh, ss;
   uint32_t heads, share, rows, seqs, cap, causal;
   float scale;
-  uint32_t tiles;
+  uint32_t tiles, pairs, pad;
   uint32_t len[NB], cnt[NB];
 };
 
@@ -542,9 +549,7 @@ TensorData Resolver::run_attend(const NodeP& n) {
   const size_t R = n->shape.size(), rows = n->shape[R - 2], heads = n->shape[R - 3];
   if (!out.layout.numel()) return out;
   const size_t nb = room_for(c.seqs), share = heads / c.heads, tiles = (share * rows + 15) / 16;
-  wkf_props props;
-  if (wkf_device_props(dev_, &props) != WKF_OK) throw Error(WKF_ERR_HIP, wkf_last_error());
-  const size_t cus = size_t(std::max(1, props.compute_units));
+  const size_t cus = compute_units(dev_);
   // Many rows take the kernel that spreads the codes in the LDS for 128 of them; it does not split a cache over workgroups, which
   // the kernel for tiles of 16 rows does.  What counts is how many full tiles of the longest sequence's length all rows come
   // to, each by its own sequence: rows behind a count are no work, and one token over a long cache is one row of a tile that
@@ -584,6 +589,7 @@ TensorData Resolver::run_attend(const NodeP& n) {
       a.causal = args.causal;
       a.scale = args.scale;
       a.tiles = uint32_t(big);
+      a.pairs = c.dp <= 128 && h && big * c.heads * c.seqs <= 2 * cus;
       std::copy(c.len.begin(), c.len.end(), a.len);
       std::copy(args.counts.begin(), args.counts.end(), a.cnt);
       launch("attend_prompt", psig, detail({{"sequences", c.seqs}, {"heads", heads}, {"kv_heads", c.heads}, {"rows", rows}, {"dim", c.dim}}), pk, grid_dim(big * c.heads * c.seqs, "attend"), 1, 1, 256, a);
