@@ -717,7 +717,7 @@ def test_attend_of_a_chunk_beside_single_tokens(gpu, case, causal, dtype):
 
 
 # so many rows of like sequences that tiles of 128 fill the chip
-FULL_CASES = [([150, 0, 129, 200], [129, 0, 129, 129], 96, 96, 64, 64), ([100, 37, 300, 1, 128, 0], [100, 37, 100, 1, 100, 0], 150, 50, 72, 32),
+FULL_CASES = [([150, 0, 129, 200], [129, 0, 129, 129], 96, 96, 64, 64), ([100, 37, 300, 1, 128, 0], [100, 37, 100, 1, 100, 0], 165, 55, 72, 32),
               ([141, 140, 0, 270, 64, 33], [140, 140, 0, 140, 64, 33], 96, 48, 128, 128), ([260] * 4, [256] * 4, 32, 32, 128, 64), ([400, 260], [200, 200], 128, 64, 16, 32)]
 
 
@@ -736,11 +736,11 @@ def test_attend_with_full_tiles_of_large_heads(gpu, dtype, lengths, counts, head
 
 @DTYPES
 def test_attend_with_full_tiles_in_other_ways(gpu, dtype):
-    check_attend_by("attend_prompt", gpu, dtype, [150, 0, 190, 65], [70, 0, 70, 65], 192, 192, 64, 32, causal=False)
-    check_attend_by("attend_prompt", gpu, dtype, [150, 0, 190, 65], [70, 0, 70, 33], 192, 192, 64, 32)
+    check_attend_by("attend_prompt", gpu, dtype, [150, 0, 190, 65], [70, 0, 70, 65], 216, 216, 64, 32, causal=False)
+    check_attend_by("attend_prompt", gpu, dtype, [150, 0, 190, 65], [70, 0, 70, 33], 216, 216, 64, 32)
     check_attend_by("attend_prompt", gpu, dtype, [150, 0, 190, 65], [64, 0, 100, 65], 192, 96, 64, 64, causal=False)
     for scale in (0.0, 4.0):
-        check_attend_by("attend_prompt", gpu, dtype, [150, 10, 190, 65], [70, 10, 70, 65], 192, 192, 64, 64, scale=scale)
+        check_attend_by("attend_prompt", gpu, dtype, [150, 10, 190, 65], [70, 10, 70, 65], 216, 216, 64, 64, scale=scale)
 
 
 # ---- without roundings to f16 on the way -----------------------------------------------------------------------------------

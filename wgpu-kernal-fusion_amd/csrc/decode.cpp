@@ -553,11 +553,12 @@ TensorData Resolver::run_attend(const NodeP& n) {
   // Many rows take the kernel that spreads the codes in the LDS for 128 of them; it does not split a cache over workgroups, which
   // the kernel for tiles of 16 rows does.  What counts is how many full tiles of the longest sequence's length all rows come
   // to, each by its own sequence: rows behind a count are no work, and one token over a long cache is one row of a tile that
-  // walks all of it alone (2048 new tokens beside 15 single ones over 32768, 32/8 heads of 128 in f16: 35 such tiles, 431 us
-  // in tiles of 16 rows and 1408 in tiles of 128; beside 15 over 2000: 516, 285 and 228).  The two meet at about 145 of them in f16
-  // (new tokens after 3500, 32/8 heads of 128: 512, which are 128, 89 and 101; 768 after 3072, 192, 132 and 113), at 190 where a tile
-  // takes a compute unit alone (f32, heads of 128: 768 tokens 262 and 261, 1024 tokens 350 and 277), and at a thousand where the
-  // registers do not hold its sums (f16, heads of 256: 2048 after 2048, 512 of them, 541 and 591; four prompts of 2048: 995 and 889).
+  // walks all of it alone (2048 new tokens beside 15 single ones over 32768, 32/8 heads of 128 in f16: 36 such tiles, 427 us
+  // in tiles of 16 rows and 1408 in tiles of 128; beside 15 over 2000: 516, 275 and 215).  The two meet at about 140 of them in
+  // f16 (new tokens up to 4096, 32/8 heads of 128: 512, which are 128 tiles, 90 and 104 us; 640, 160, 108 and 104; 768, 192, 126 and
+  // 105), at 175 with heads of 192 (145 and 155; 169 and 156), and at 220 where a tile takes a compute unit alone (f32, heads of
+  // 128: 768 tokens 244 and 269, 896, 224, 273 and 268) or the registers do not hold its sums (f16, heads of 256: 1024 tokens,
+  // 256, 358 and 326).
   double work = 0;
   size_t furthest = 0;
   for (size_t b = 0; b < c.seqs; b++) {
@@ -566,7 +567,7 @@ TensorData Resolver::run_attend(const NodeP& n) {
     furthest = std::max<size_t>(furthest, c.len[b]);
   }
   const bool h = n->dtype == DType::F16;
-  const double full = double(cus) * (!h ? 0.75 : c.dp <= 128 ? 0.5625 : c.dp <= 192 ? 0.75 : 4.0);
+  const double full = double(cus) * (!h ? 0.875 : c.dp <= 128 ? 0.5625 : c.dp <= 192 ? 0.75 : 1.0);
   const size_t big = (share * rows + 127) / 128;
   if (share * rows > 64 && furthest && work >= full * 128 * double(furthest)) {
     const size_t weight_parts = !h ? 3 : st_.exact_math ? 2 : 1;
