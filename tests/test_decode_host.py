@@ -5,6 +5,7 @@ import os
 import re
 import shutil
 import subprocess
+import sys
 
 import numpy as np
 import pytest
@@ -322,6 +323,74 @@ def test_extern_block_of_the_guide_matches_the_header():
     block = block[:block.index("```")]
     rust = {m.group(1): len([p for p in m.group(2).split(",") if p.strip()]) for m in re.finditer(r"pub fn (wkf_\w+)\s*\(([^)]*)\)", block)}
     assert rust == c
+
+
+KERNELS = r"""
+import sys
+import numpy as np
+sys.path.insert(0, TESTS)
+from helpers import load_package
+w = load_package()
+dev = w.Device.planner()
+T, H, F = w.Tensor, np.float16, np.float32
+seen = set()
+def done(t):
+    t.materialize()
+    seen.update(k.signature for k in t.kernels())
+for k, n, ms in ((136, 200, (1, 24, 33)), (160, 2000, (300, 600, 1100)), (130, 7000, (600,)), (64, 11008, (800,))):
+    for group in (32, 64, 128):
+        for zeros in (None, np.zeros((-(-k // group), n), np.uint8)):
+            q4 = w.Q4Weights(dev, np.zeros((k, n), np.uint8), np.ones((-(-k // group), n), H), zeros, group)
+            for m in ms:
+                for dt in (H, F):
+                    done(T.new(dev, np.zeros((m, k), dt)).mat_mul_q4(q4))
+for dim in (20, 64, 128, 192, 255, 256):
+    for dt in (H, F):
+        cache = w.KvCache(dev, 1, 256, dim, 192, 128)
+        t = T.new(dev, np.zeros((1, 256, 150, dim), dt))
+        cache.append(t, t)
+        for q in (t, t.narrow(2, 0, 3), t.narrow(2, 0, 20)):
+            done(q.attend(cache))
+        done(cache.values(0, 150, w.F16 if dt == H else w.F32))
+for dim in (6, 128, 1024):
+    for dt in (H, F):
+        c = T.new(dev, np.zeros((9, dim), F))
+        done(T.new(dev, np.zeros((2, 5, dim), dt)).norm_rope(T.new(dev, np.zeros(dim, dt)), c, c, 1e-5))
+print("\n".join(sorted(seen)))
+"""
+
+
+def test_decoder_kernels_use_no_scratch_memory(tmp_path):
+    """The compiler's own record of every kernel of these operators: no private segment and no spilled vector register, but for
+    two that do not fit: tiles of 128 rows with heads above 192 elements, and the larger tiles of a 4-bit product of f16 rows with
+    scales for 32 or 64 rows."""
+    from test_host_abi import _code_object_kernels
+
+    def entry(signature):
+        h = 1469598103934665603
+        for c in signature.encode():
+            h = (h ^ c) * 1099511628211 & (1 << 64) - 1
+        return f"wkf_{signature.split('|')[0]}_{(h ^ h >> 32) & 0xffffffff:08x}"
+
+    def known(signature):
+        dim = re.search(r"^attend_prompt\|.*\|d(\d+)\|", signature)
+        return bool(dim and int(dim.group(1)) > 192 or re.search(r"^q4_tile\|gfx950\|f16\|.*\|step[12]\|.*(4x4x8x1|2x2x4x4)$", signature))
+
+    r = subprocess.run([sys.executable, "-c", f"TESTS = {os.path.join(ROOT, 'tests')!r}\n" + KERNELS], capture_output=True, text=True, timeout=900, env=dict(os.environ, WKF_CACHE_DIR=str(tmp_path)))
+    assert r.returncode == 0, r.stderr
+    names = {entry(s): s for s in r.stdout.split("\n") if s}
+    spilled, checked = [], set()
+    for path in tmp_path.glob("*.hsaco"):
+        for k in _code_object_kernels(path):
+            name = k[".name"]
+            if not re.match(r"wkf_(q4_|attend_|kv_|norm_rope)", name):
+                continue
+            checked.add(name.rsplit("_", 1)[0])
+            if (k[".private_segment_fixed_size"] or k[".vgpr_spill_count"] or k[".uses_dynamic_stack"]) and not known(names.get(name, "")):
+                spilled.append((names.get(name, name), k[".private_segment_fixed_size"], k[".vgpr_spill_count"]))
+            assert k[".vgpr_count"] <= 512
+    assert not spilled, spilled
+    assert checked == {"wkf_" + k for k in ("q4_pack", "q4_rows", "q4_tile", "q4_mat_mul", "q4_dense", "attend_rows", "attend_prompt", "kv_append", "kv_values", "norm_rope")}, checked
 
 
 FACADE = r"""
