@@ -35,7 +35,7 @@ int wkf_tensor_zeros(wkf_device* dev, int dtype, int rank, const size_t* shape, 
  * the same shape, dtype and device; one pass over the joint graph, as wkf_tensor_materialize_many.  An output may be a
  * leaf of any of the graphs: every value is computed from what the leaves held before the call.  The launches are
  * recorded on ts[0].  Tensors recorded earlier that have outs[i] among their leaves see the new values when they are
- * materialised next.  No two outputs may be the same tensor. */
+ * materialised next.  No two outputs may be the same tensor.  When it fails, some outputs may hold their new values already. */
 int wkf_tensor_materialize_into(wkf_tensor* const* ts, int n, wkf_tensor* const* outs);
 /* The device address of the first element of a tensor that holds data.  What has been launched on the device may still
  * be writing there: wkf_device_sync first.  The address is good until the last handle of the tensor is freed. */
@@ -94,7 +94,8 @@ int wkf_kv_cache_values(wkf_kv_cache* c, int dtype, size_t first, size_t count, 
  * softmax(scale q k^T) v.  Head h reads key head h / (heads / kv_heads).  The S rows are the LAST tokens of each sequence, or
  * its last counts[b] <= S ones (then rows behind counts[b] give zeros); with causal != 0 a row sees the tokens up to its own,
  * else all of its sequence.  A row that sees no token gives zeros.  scale is finite and not negative.
- * With more than 16 rows of f16 for a key head its softmax weights may be rounded to f16 (never with exact math).
+ * With more than 16 rows of f16 for a key head its softmax weights may be rounded to f16 (never with exact math).  Weighted values
+ * are summed in f32 before they are divided by the sum of the weights: values beyond 3.4e38 / tokens may overflow.
  * The node stands for the cache as it is now: materialising it after an append or a reset is WKF_ERR_INVALID_ARG. */
 int wkf_tensor_attend(const wkf_tensor* q, wkf_kv_cache* c, float scale, int causal, const size_t* counts, wkf_tensor** out);
 

@@ -138,9 +138,9 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
   const size_t cus = compute_units(dev_);
   auto tiles_of = [&](size_t mt, size_t columns) { return (M + 16 * mt - 1) / (16 * mt) * ((w.tiles_n() + columns - 1) / columns); };
   // Many f16 rows: where no tiles below cover the product with one round of the chip, the weights are written out once, each
-  // rounded to f16, and the product is mat_mul's ([1024,4096]x[4096,11008]: 114 us against 122 in tiles of 4-bit weights;
+  // rounded to f16, and the product is mat_mul's ([1024,4096]x[4096,11008]: 114 us against 130 in tiles of 4-bit weights;
   // [1024,11008]x[11008,4096], which one round covers: 154 against 104).  Weights that would overflow or lose bits in f16
-  // stay in the tiles, which round none, and so does everything where the caller wants exact math ([1024,4096]x[4096,11008]: 128).
+  // stay in the tiles, which round none, and so does everything where the caller wants exact math.
   if (h && w.fits_f16 && !st_.exact_math && M >= 768 && tiles_of(4, 32) > cus && w.tiles_n() <= 65535) return mat_mul_q4_dense(w, x, out, M);
   // the k = 32 steps of a tile that surely share a group, and the group in units of so many
   const size_t step = w.group % 128 == 0 ? 4 : w.group % 64 == 0 ? 2 : 1, units = w.group / (32 * step);
@@ -150,11 +150,11 @@ TensorData Resolver::run_mat_mul_q4(const NodeP& n) {
   const std::string kind = joined({dtype_name(x.dtype), "|s", dtype_name(w.scale_dtype), z ? "|zeros" : "", "|step", step, shift < 0 ? "|any" : ""});
   auto defines = [&] { return define("WKF_H", h) + define("WKF_SH", w.scale_dtype == DType::F16) + define("WKF_Z", z) + define("STEP", step) + define("POW2", shift >= 0); };
   const std::string d = detail({{"m", M}, {"n", N}, {"k", w.k}, {"group", w.group}});
-  // More than 16 rows share x in the LDS; up to 32 beside few columns do not pay for it (24 rows of [4096,4096]: 9.5 us against 12.4).
+  // More than 16 rows share x in the LDS; up to 32 beside few columns do not pay for it (24 rows of [4096,4096]: 10.4 us against 11.3).
   if (M > (w.tiles_n() <= cus ? 32 : 16)) {
     // The smallest tiles of which the chip takes all at once, one a compute unit: larger ones read x less often, smaller ones
-    // have K shared by more groups of waves ([4096,4096] f16: 256 rows 19.7 us in 32 x 128, 28.7 in 32 x 64, 28.3 in 64 x 128;
-    // 1024 rows 42 in 64 x 256, 54 in 64 x 128; f32 256 rows 46 in 32 x 128, 70 in 32 x 64, 67 in 32 x 256).
+    // have K shared by more groups of waves ([4096,4096] f16: 256 rows 16.7 us in 32 x 128, 24.9 in 32 x 64, 26.5 in 64 x 128;
+    // 1024 rows 41 in 64 x 256, 51 in 64 x 128; f32 256 rows 43 in 32 x 128, 65 in 32 x 64, 65 in 32 x 256).
     struct Tile {
       size_t mt, nt, nw, kw;
     };
